@@ -5,13 +5,15 @@ import sys
 
 import flash_window_attention_v2_amd as _impl
 from flash_window_attention_v2_amd import (FlashWindowAttentionV2, FlashWindowAttentionV2Grid,
-                                           FlashWindowAttentionV2QKVPacked, SwinTransformerV2, WindowAttention,
-                                           flash_win_attn_v2_func, flash_win_attn_v2_grid_func,
-                                           flash_win_attn_v2_qkvpacked_func, win_attention_torch,
-                                           win_attention_torch_compile)
-from flash_window_attention_v2_amd import flash_window_attention_v2, kernels, swin_transformer_v2, win_attention_func
+                                           FlashWindowAttentionV2QKVPacked, FusedLinear, ResidualNorm, SwinTransformerV2,
+                                           WindowAttention, flash_win_attn_v2_func, flash_win_attn_v2_grid_func,
+                                           flash_win_attn_v2_qkvpacked_func, fused_linear_fp8_func, fused_linear_func,
+                                           quantize_rows_func, residual_norm_fp8_func, residual_norm_func,
+                                           win_attention_torch, win_attention_torch_compile)
+from flash_window_attention_v2_amd import (block_ops, flash_window_attention_v2, kernels, swin_transformer_v2,
+                                           win_attention_func)
 
-for _name in ("flash_window_attention_v2", "kernels", "swin_transformer_v2", "win_attention_func"):
+for _name in ("block_ops", "flash_window_attention_v2", "kernels", "swin_transformer_v2", "win_attention_func"):
     sys.modules[__name__ + "." + _name] = getattr(_impl, _name)
 
 __all__ = _impl.__all__

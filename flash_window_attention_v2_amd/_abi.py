@@ -12,8 +12,12 @@ import threading
 ABI_VERSION = 4
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_HIP, ERR_NO_DEVICE = range(5)
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3 = 0, 1, 2, 3
 SCALE_DEFAULT, SCALE_TENSOR = 0, 1
+ACT_NONE, ACT_GELU, ACT_GELU_TANH, ACT_SILU, ACT_RELU = range(5)
+NORM_LAYER, NORM_RMS = 0, 1
+NORM_POST, NORM_PRE = 0, 1
+NORM_MAX_DIM = 16384                # FWA2_NORM_MAX_DIM of include/fwa2.h
 STATIC_SCRATCH_BYTES = 128 << 20    # FWA2_STATIC_SCRATCH_BYTES of include/fwa2.h
 MASK_REGION_BYTES = 272             # FWA2_MASK_REGION_BYTES of include/fwa2.h
 
@@ -31,6 +35,15 @@ EXPORTS = (
     "fwa2_backward_static",
     "fwa2_cpb_bias_forward",
     "fwa2_cpb_bias_backward",
+    "fwa2_norm_validate",
+    "fwa2_norm_workspace_bytes",
+    "fwa2_norm_forward",
+    "fwa2_norm_backward",
+    "fwa2_quantize_rows",
+    "fwa2_linear_validate",
+    "fwa2_linear_workspace_bytes",
+    "fwa2_linear_forward",
+    "fwa2_linear_backward",
 )
 
 
@@ -64,6 +77,43 @@ class Problem(ctypes.Structure):
         ("n_keys", ctypes.c_int32), ("scale_head_dim", ctypes.c_int32),
         ("mask_regions", ctypes.c_void_p),
         ("ev_start", ctypes.c_void_p), ("ev_stop", ctypes.c_void_p),
+    ]
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", ctypes.c_uint32), ("abi_version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32), ("stream_dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32),
+        ("kind", ctypes.c_int32), ("placement", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("rows", ctypes.c_int64), ("dim", ctypes.c_int32), ("gate_dtype", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("shortcut", ctypes.c_void_p), ("shortcut_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p), ("rows_per_gate", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("h", ctypes.c_void_p), ("y8", ctypes.c_void_p), ("y8_scale", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64), ("dh", ctypes.c_void_p), ("dh_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("dshortcut", ctypes.c_void_p), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class Linear(ctypes.Structure):
+    _fields_ = [
+        ("struct_bytes", ctypes.c_uint32), ("abi_version", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+        ("in_features", ctypes.c_int32), ("out_features", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("weight_stride", ctypes.c_int64),
+        ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p), ("weight_scale", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("z", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
     ]
 
 
@@ -116,6 +166,19 @@ def load():
         lib.fwa2_cpb_bias_backward.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]
         lib.fwa2_cpb_bias_backward.restype = ctypes.c_int
+        lib.fwa2_norm_validate.argtypes = [ctypes.POINTER(Norm), ctypes.c_int]
+        lib.fwa2_norm_workspace_bytes.argtypes = [ctypes.POINTER(Norm)]
+        lib.fwa2_norm_workspace_bytes.restype = ctypes.c_size_t
+        lib.fwa2_norm_forward.argtypes = lib.fwa2_norm_backward.argtypes = [ctypes.POINTER(Norm)]
+        lib.fwa2_quantize_rows.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        lib.fwa2_linear_validate.argtypes = [ctypes.POINTER(Linear), ctypes.c_int]
+        lib.fwa2_linear_workspace_bytes.argtypes = [ctypes.POINTER(Linear), ctypes.c_int]
+        lib.fwa2_linear_workspace_bytes.restype = ctypes.c_size_t
+        lib.fwa2_linear_forward.argtypes = lib.fwa2_linear_backward.argtypes = [ctypes.POINTER(Linear)]
+        for name in ("fwa2_norm_validate", "fwa2_norm_forward", "fwa2_norm_backward", "fwa2_quantize_rows",
+                     "fwa2_linear_validate", "fwa2_linear_forward", "fwa2_linear_backward"):
+            getattr(lib, name).restype = ctypes.c_int
         if lib.fwa2_abi_version() != ABI_VERSION:
             raise Fwa2Error(f"libfwa2 ABI {lib.fwa2_abi_version()} != binding ABI {ABI_VERSION}")
         _lib = lib
@@ -125,6 +188,20 @@ def load():
 def new_problem():
     p = Problem()
     p.struct_bytes = ctypes.sizeof(Problem)
+    p.abi_version = ABI_VERSION
+    return p
+
+
+def new_norm():
+    p = Norm()
+    p.struct_bytes = ctypes.sizeof(Norm)
+    p.abi_version = ABI_VERSION
+    return p
+
+
+def new_linear():
+    p = Linear()
+    p.struct_bytes = ctypes.sizeof(Linear)
     p.abi_version = ABI_VERSION
     return p
 

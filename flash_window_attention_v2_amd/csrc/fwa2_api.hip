@@ -2,6 +2,7 @@
 // validation, workspace sizing and dispatch to the gfx950 kernels.  Nothing
 // here allocates device memory or synchronises.
 #include <atomic>
+#include <math.h>
 #include <mutex>
 #include <stdarg.h>
 #include <stdio.h>
@@ -24,6 +25,14 @@ int backward_supported(int n);
 hipError_t launch_cpb_bias_forward(const void* table, int dtype, int heads, int wh, int ww, void* bias, hipStream_t st);
 hipError_t launch_cpb_bias_backward(const void* table, const void* dbias, int dtype, int heads, int wh, int ww,
                                     void* dtable, hipStream_t st);
+hipError_t launch_norm_forward(const fwa2_norm* p, int cus, hipStream_t st);
+hipError_t launch_norm_backward(const fwa2_norm* p, int cus, hipStream_t st);
+size_t norm_workspace_bytes(const fwa2_norm* p, int cus);
+hipError_t launch_quantize_rows(const void* x, int dtype, int64_t rows, int dim, int64_t xs, void* q, float* scale, hipStream_t st);
+hipError_t launch_linear_forward(const fwa2_linear* p, int cus, hipStream_t st);
+hipError_t launch_linear_backward(const fwa2_linear* p, int cus, hipStream_t st);
+size_t linear_workspace_bytes(const fwa2_linear* p, bool backward, int cus);
+bool linear_fits(const fwa2_linear* p);
 }  // namespace fwa2
 
 namespace {
@@ -393,6 +402,221 @@ int fwa2_backward_static(const fwa2_problem* p) {
     q.workspace = ptr;
     q.workspace_bytes = kStaticScratchBytes;
     return run_backward(&q);
+}
+
+// ---- normalisation, 8-bit rows, matrix products ----
+static int check_layout(const char* what, uint32_t bytes, uint32_t abi, size_t want) {
+    if (bytes != want || abi != FWA2_ABI_VERSION)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "%s layout mismatch: caller %u bytes / abi %u, library %zu bytes / abi %d", what,
+                    bytes, abi, want, FWA2_ABI_VERSION);
+    return FWA2_OK;
+}
+
+// Sizes alone, which is what the workspace depends on.
+static int check_norm_sizes(const fwa2_norm* p) {
+    if (p->rows < 1 || p->rows > 0x7fffffffLL || p->dim < 1)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: rows must be 1 .. 2^31 - 1 and dim positive");
+    if (p->dim > FWA2_NORM_MAX_DIM)
+        return fail(FWA2_ERR_UNSUPPORTED, "norm: rows of %d values, at most %d are supported", p->dim, FWA2_NORM_MAX_DIM);
+    return FWA2_OK;
+}
+
+static int check_rows(const char* name, const void* ptr, int64_t stride, int64_t len, size_t elem) {
+    if (ptr == nullptr) return fail(FWA2_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+    if (reinterpret_cast<uintptr_t>(ptr) % elem) return fail(FWA2_ERR_INVALID_ARGUMENT, "%s: pointer is not a multiple of its element size", name);
+    if (stride < len) return fail(FWA2_ERR_INVALID_ARGUMENT, "%s: row stride %lld overlaps rows", name, (long long)stride);
+    return FWA2_OK;
+}
+static int check_ptr(const char* name, const void* ptr, size_t elem) { return check_rows(name, ptr, 0, 0, elem); }
+
+static int validate_norm(const fwa2_norm* p, int backward) {
+    if (p == nullptr) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm description is null");
+    int rc = check_layout("fwa2_norm", p->struct_bytes, p->abi_version, sizeof(fwa2_norm));
+    if (rc) return rc;
+    if (p->dtype != FWA2_F16 && p->dtype != FWA2_BF16 && p->dtype != FWA2_F32)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: dtype must be fp16, bf16 or fp32");
+    if ((p->stream_dtype != p->dtype && p->stream_dtype != FWA2_F32) || (p->param_dtype != p->dtype && p->param_dtype != FWA2_F32))
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: stream_dtype and param_dtype must be dtype or fp32");
+    if (p->kind != FWA2_NORM_LAYER && p->kind != FWA2_NORM_RMS) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: kind %d unknown", p->kind);
+    const bool pre = p->placement == FWA2_NORM_PRE;
+    if (!pre && p->placement != FWA2_NORM_POST) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: placement %d unknown", p->placement);
+    if (!(p->eps > 0.f && p->eps < INFINITY)) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: eps must be positive");
+    if ((rc = check_norm_sizes(p))) return rc;
+    const size_t xb = p->dtype == FWA2_F32 ? 4 : 2, sb = p->stream_dtype == FWA2_F32 ? 4 : 2, wb = p->param_dtype == FWA2_F32 ? 4 : 2;
+    const size_t yb = pre ? xb : sb;
+    if ((rc = check_ptr("weight", p->weight, wb))) return rc;
+    if (p->bias && (rc = check_ptr("bias", p->bias, wb))) return rc;
+    if (p->gate) {
+        if (p->gate_dtype != p->dtype && p->gate_dtype != FWA2_F32)
+            return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: gate must be of dtype or fp32");
+        if ((rc = check_ptr("gate", p->gate, p->gate_dtype == FWA2_F32 ? 4 : 2))) return rc;
+        if (p->rows_per_gate < 1 || p->rows_per_gate > p->rows || p->rows % p->rows_per_gate)
+            return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: %lld rows are no multiple of rows_per_gate %lld", (long long)p->rows,
+                        (long long)p->rows_per_gate);
+    }
+    if (!backward) {
+        if ((rc = check_rows("x", p->x, p->x_stride, p->dim, xb))) return rc;
+        if (pre && p->shortcut == nullptr) return fail(FWA2_ERR_INVALID_ARGUMENT, "shortcut: null in the pre-norm form");
+        if (p->shortcut && (rc = check_rows("shortcut", p->shortcut, p->shortcut_stride, p->dim, sb))) return rc;
+        if (pre && (rc = check_ptr("h", p->h, sb))) return rc;
+        if (!(pre && p->y8) && p->y == nullptr) return fail(FWA2_ERR_INVALID_ARGUMENT, "y: null pointer");
+        if (p->y && (rc = check_ptr("y", p->y, yb))) return rc;
+        if (p->y8 && (rc = check_ptr("y8_scale", p->y8_scale, 4))) return rc;
+        if (p->stats && (rc = check_ptr("stats", p->stats, 8))) return rc;
+        return FWA2_OK;
+    }
+    if (pre) {
+        if ((rc = check_ptr("h", p->h, sb))) return rc;
+        if (p->dy && (rc = check_rows("dy", p->dy, p->dy_stride, p->dim, yb))) return rc;
+        if (p->dh && (rc = check_rows("dh", p->dh, p->dh_stride, p->dim, sb))) return rc;
+        if (p->dshortcut && (rc = check_ptr("dshortcut", p->dshortcut, sb))) return rc;
+    } else {
+        if ((rc = check_rows("x", p->x, p->x_stride, p->dim, xb))) return rc;
+        if ((rc = check_rows("dy", p->dy, p->dy_stride, p->dim, yb))) return rc;
+        if (p->dshortcut) return fail(FWA2_ERR_INVALID_ARGUMENT, "dshortcut: the post-norm form has none of its own (it is dy)");
+    }
+    if ((rc = check_ptr("stats", p->stats, 8))) return rc;
+    if (p->dx && (rc = check_ptr("dx", p->dx, xb))) return rc;
+    if (p->dweight && (rc = check_ptr("dweight", p->dweight, wb))) return rc;
+    if (p->dbias && (rc = check_ptr("dbias", p->dbias, wb))) return rc;
+    const size_t need = fwa2::norm_workspace_bytes(p, cu_count());
+    if (need && (p->workspace == nullptr || p->workspace_bytes < need))
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "workspace: need %zu bytes, got %zu", need, p->workspace_bytes);
+    if (need && !aligned16(p->workspace)) return fail(FWA2_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    return FWA2_OK;
+}
+
+int fwa2_norm_validate(const fwa2_norm* p, int backward) {
+    g_err[0] = 0;
+    return validate_norm(p, backward);
+}
+
+size_t fwa2_norm_workspace_bytes(const fwa2_norm* p) {
+    if (p == nullptr || p->rows < 1 || p->rows > 0x7fffffffLL || p->dim < 1 || p->dim > FWA2_NORM_MAX_DIM) return 0;
+    return fwa2::norm_workspace_bytes(p, cu_count());
+}
+
+int fwa2_norm_forward(const fwa2_norm* p) {
+    g_err[0] = 0;
+    const int rc = validate_norm(p, 0);
+    if (rc) return rc;
+    const hipError_t e = fwa2::launch_norm_forward(p, cu_count(), (hipStream_t)p->stream);
+    if (e != hipSuccess) return fail(FWA2_ERR_HIP, "norm forward launch: %s", hipGetErrorString(e));
+    return FWA2_OK;
+}
+
+int fwa2_norm_backward(const fwa2_norm* p) {
+    g_err[0] = 0;
+    const int rc = validate_norm(p, 1);
+    if (rc) return rc;
+    if (!p->dx && !p->dshortcut && !p->dweight && !p->dbias) return FWA2_OK;
+    const hipError_t e = fwa2::launch_norm_backward(p, cu_count(), (hipStream_t)p->stream);
+    if (e != hipSuccess) return fail(FWA2_ERR_HIP, "norm backward launch: %s", hipGetErrorString(e));
+    return FWA2_OK;
+}
+
+int fwa2_quantize_rows(const void* x, int dtype, int64_t rows, int dim, int64_t x_stride, void* q, float* scale, void* stream) {
+    g_err[0] = 0;
+    if (dtype != FWA2_F16 && dtype != FWA2_BF16 && dtype != FWA2_F32)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "quantize_rows: dtype must be fp16, bf16 or fp32");
+    if (rows < 1 || rows > 0x7fffffffLL || dim < 1)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "quantize_rows: rows must be 1 .. 2^31 - 1 and dim positive");
+    if (dim > FWA2_NORM_MAX_DIM)
+        return fail(FWA2_ERR_UNSUPPORTED, "quantize_rows: rows of %d values, at most %d are supported", dim, FWA2_NORM_MAX_DIM);
+    int rc;
+    if ((rc = check_rows("x", x, x_stride, dim, dtype == FWA2_F32 ? 4 : 2)) || (rc = check_ptr("q", q, 1)) || (rc = check_ptr("scale", scale, 4)))
+        return rc;
+    const hipError_t e = fwa2::launch_quantize_rows(x, dtype, rows, dim, x_stride, q, scale, (hipStream_t)stream);
+    if (e != hipSuccess) return fail(FWA2_ERR_HIP, "quantize_rows launch: %s", hipGetErrorString(e));
+    return FWA2_OK;
+}
+
+static int check_linear_sizes(const fwa2_linear* p) {
+    if (p->rows < 1 || p->rows > 0x7fffffffLL || p->in_features < 1 || p->out_features < 1)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "linear: rows must be 1 .. 2^31 - 1, in_features and out_features positive");
+    if (p->in_features >= (1 << 24) || p->out_features >= (1 << 24) || !fwa2::linear_fits(p))
+        return fail(FWA2_ERR_UNSUPPORTED, "linear: %lld x %d x %d is too large for one launch", (long long)p->rows, p->in_features, p->out_features);
+    return FWA2_OK;
+}
+
+static int check_matrix(const char* name, const void* ptr, int64_t stride, int64_t len, size_t elem) {
+    const int rc = check_rows(name, ptr, stride, len, elem);
+    if (rc) return rc;
+    // rows inside a tile are addressed with 32-bit offsets
+    if (stride >= (1 << 22)) return fail(FWA2_ERR_UNSUPPORTED, "%s: row stride %lld is beyond 2^22 elements", name, (long long)stride);
+    return FWA2_OK;
+}
+
+static int validate_linear(const fwa2_linear* p, int backward) {
+    if (p == nullptr) return fail(FWA2_ERR_INVALID_ARGUMENT, "linear description is null");
+    int rc = check_layout("fwa2_linear", p->struct_bytes, p->abi_version, sizeof(fwa2_linear));
+    if (rc) return rc;
+    if (p->dtype != FWA2_F16 && p->dtype != FWA2_BF16) return fail(FWA2_ERR_INVALID_ARGUMENT, "linear: Only support fp16 and bf16");
+    if (p->x_dtype != p->dtype && p->x_dtype != FWA2_E4M3)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "linear: x and weight must be of dtype or e4m3");
+    if (p->activation < FWA2_ACT_NONE || p->activation > FWA2_ACT_RELU)
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "linear: activation %d unknown", p->activation);
+    if ((rc = check_linear_sizes(p))) return rc;
+    const bool f8 = p->x_dtype == FWA2_E4M3;
+    const size_t xb = f8 ? 1 : 2;
+    if (backward && f8) return fail(FWA2_ERR_UNSUPPORTED, "linear: 8-bit products have no backward pass");
+    if ((!backward || p->dweight) && (rc = check_matrix("x", p->x, p->x_stride, p->in_features, xb))) return rc;
+    if ((!backward || p->dx) && (rc = check_matrix("weight", p->weight, p->weight_stride, p->in_features, xb))) return rc;
+    if (!backward) {
+        if (p->bias && (rc = check_ptr("bias", p->bias, 2))) return rc;
+        if (p->residual && (rc = check_matrix("residual", p->residual, p->residual_stride, p->out_features, 2))) return rc;
+        if (f8 && ((rc = check_ptr("x_scale", p->x_scale, 4)) || (rc = check_ptr("weight_scale", p->weight_scale, 4)))) return rc;
+        if ((rc = check_ptr("y", p->y, 2))) return rc;
+        if (p->z && (rc = check_ptr("z", p->z, 2))) return rc;
+    } else {
+        if ((rc = check_matrix("dy", p->dy, p->dy_stride, p->out_features, 2))) return rc;
+        if (p->activation != FWA2_ACT_NONE) {
+            if ((rc = check_ptr("z", p->z, 2))) return rc;
+            // dz has rows of out_features
+            if (p->out_features >= (1 << 22)) return fail(FWA2_ERR_UNSUPPORTED, "linear: out_features is beyond 2^22");
+        }
+        if (p->dx && (rc = check_ptr("dx", p->dx, 2))) return rc;
+        if (p->dweight && (rc = check_ptr("dweight", p->dweight, 2))) return rc;
+        if (p->dbias && !p->dweight) return fail(FWA2_ERR_INVALID_ARGUMENT, "dbias: wanted without dweight");
+        if (p->dbias && (rc = check_ptr("dbias", p->dbias, 2))) return rc;
+    }
+    const size_t need = fwa2::linear_workspace_bytes(p, backward != 0, cu_count());
+    if (need && (p->workspace == nullptr || p->workspace_bytes < need))
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "workspace: need %zu bytes, got %zu", need, p->workspace_bytes);
+    if (need && (reinterpret_cast<uintptr_t>(p->workspace) & 255))
+        return fail(FWA2_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    return FWA2_OK;
+}
+
+int fwa2_linear_validate(const fwa2_linear* p, int backward) {
+    g_err[0] = 0;
+    return validate_linear(p, backward);
+}
+
+size_t fwa2_linear_workspace_bytes(const fwa2_linear* p, int backward) {
+    if (p == nullptr) return 0;
+    const int rc = check_linear_sizes(p);
+    g_err[0] = 0;       // a query leaves no error behind
+    return rc ? 0 : fwa2::linear_workspace_bytes(p, backward != 0, cu_count());
+}
+
+int fwa2_linear_forward(const fwa2_linear* p) {
+    g_err[0] = 0;
+    const int rc = validate_linear(p, 0);
+    if (rc) return rc;
+    const hipError_t e = fwa2::launch_linear_forward(p, cu_count(), (hipStream_t)p->stream);
+    if (e != hipSuccess) return fail(FWA2_ERR_HIP, "linear forward launch: %s", hipGetErrorString(e));
+    return FWA2_OK;
+}
+
+int fwa2_linear_backward(const fwa2_linear* p) {
+    g_err[0] = 0;
+    const int rc = validate_linear(p, 1);
+    if (rc) return rc;
+    if (!p->dx && !p->dweight) return FWA2_OK;
+    const hipError_t e = fwa2::launch_linear_backward(p, cu_count(), (hipStream_t)p->stream);
+    if (e != hipSuccess) return fail(FWA2_ERR_HIP, "linear backward launch: %s", hipGetErrorString(e));
+    return FWA2_OK;
 }
 
 }  // extern "C"

@@ -293,6 +293,151 @@ int fwa2_cpb_bias_forward(const void* table, int dtype, int heads, int wh, int w
 int fwa2_cpb_bias_backward(const void* table, const void* dbias, int dtype, int heads, int wh, int ww, void* dtable,
                            void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * The rest of a transformer block: normalisation with the residual's addition, matrix products with an epilogue, and
+ * the 8-bit forms of both.  The reference composes these from framework calls (nn.LayerNorm, nn.Linear, nn.GELU and
+ * the additions of flash_win_attn_v2/swin_transformer_v2.py:66-85, 443-445).  The conventions at the top of this file
+ * hold; rows are the flattened leading dimensions of a tensor, their innermost stride is 1, and
+ * both extents of a matrix are at most 2^24 - 1 (weights) respectively 2^31 - 1 (rows).
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* 8-bit floats with 4 exponent and 3 mantissa bits, no infinities, largest value 448 (the OCP encoding). */
+#define FWA2_E4M3 3
+
+typedef enum fwa2_activation {
+    FWA2_ACT_NONE = 0,
+    FWA2_ACT_GELU = 1,      /* z Phi(z) */
+    FWA2_ACT_GELU_TANH = 2, /* z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+    FWA2_ACT_SILU = 3,      /* z / (1 + exp(-z)) */
+    FWA2_ACT_RELU = 4
+} fwa2_activation;
+
+typedef enum fwa2_norm_kind { FWA2_NORM_LAYER = 0, FWA2_NORM_RMS = 1 } fwa2_norm_kind;
+typedef enum fwa2_norm_place {
+    FWA2_NORM_POST = 0, /* y = shortcut + g norm(x)               (shortcut may be absent: y = g norm(x)) */
+    FWA2_NORM_PRE = 1   /* h = shortcut + g x, y = norm(h)        */
+} fwa2_norm_place;
+
+/*
+ * norm(v) = (v - mean) / sqrt(var + eps) * weight + bias (LAYER; var is the mean of the squared deviations) or
+ * v / sqrt(mean(v^2) + eps) * weight + bias (RMS), over the `dim` values of a row; statistics, sums and products in
+ * fp32, every output rounded once.  In the PRE form the statistics are those of the unrounded h.
+ * Types: x, dx and (PRE) y, dy are `dtype`; shortcut, (POST) y, dy, (PRE) h, dh and dshortcut are `stream_dtype`;
+ * weight, bias, dweight, dbias are `param_dtype`; stream_dtype and param_dtype are `dtype` or FWA2_F32.
+ */
+typedef struct fwa2_norm {
+    uint32_t struct_bytes;  /* sizeof(fwa2_norm) as the caller compiled it */
+    uint32_t abi_version;   /* FWA2_ABI_VERSION */
+    int32_t dtype;          /* FWA2_F16, FWA2_BF16 or FWA2_F32 */
+    int32_t stream_dtype;
+    int32_t param_dtype;
+    int32_t kind;           /* fwa2_norm_kind */
+    int32_t placement;      /* fwa2_norm_place */
+    float   eps;            /* > 0 */
+    int64_t rows;           /* 1 .. 2^31 - 1 */
+    int32_t dim;            /* 1 .. FWA2_NORM_MAX_DIM */
+    int32_t gate_dtype;     /* `dtype` or FWA2_F32 */
+
+    const void* x;          /* [rows, dim], rows x_stride elements apart; backward (PRE): not read */
+    int64_t     x_stride;
+    const void* shortcut;   /* [rows, dim]; NULL only in the POST form; backward: not read */
+    int64_t     shortcut_stride;
+    const void* weight;     /* [dim] */
+    const void* bias;       /* [dim] or NULL */
+    const void* gate;       /* one factor g per rows_per_gate consecutive rows, or NULL (g = 1) */
+    int64_t     rows_per_gate;
+
+    void*  y;               /* [rows, dim] contiguous; NULL with the 8-bit output of the PRE form */
+    void*  h;               /* PRE: [rows, dim] contiguous.  Backward: the h that the forward call wrote */
+    void*  y8;              /* optional [rows, dim] contiguous e4m3: y divided by its row's scale; forward only */
+    float* y8_scale;        /* [rows], with y8: max(max |y| of the row, 2^-100) * fp32(1 / 448) */
+    float* stats;           /* [rows, 2] mean (0 for RMS) and 1 / sqrt(..) of each row: forward writes them unless
+                               NULL, backward reads them */
+
+    /* (backward) */
+    const void* dy;         /* [rows, dim] gradient of y, or NULL = zero (PRE only) */
+    int64_t     dy_stride;
+    const void* dh;         /* PRE: gradient of h, or NULL = zero */
+    int64_t     dh_stride;
+    void* dx;               /* [rows, dim] contiguous, or NULL = not wanted */
+    void* dshortcut;        /* PRE: [rows, dim] contiguous, or NULL = not wanted.  (POST: it is dy) */
+    void* dweight;          /* [dim], or NULL = not wanted */
+    void* dbias;            /* [dim], or NULL = not wanted */
+    void* workspace;        /* fwa2_norm_workspace_bytes() bytes, 16-byte aligned, uninitialised */
+    size_t workspace_bytes;
+
+    void* stream;           /* hipStream_t */
+} fwa2_norm;
+
+#define FWA2_NORM_MAX_DIM 16384
+
+/* Checks a description without touching device memory, as fwa2_validate does for the attention. */
+int fwa2_norm_validate(const fwa2_norm* p, int backward);
+/* Scratch of fwa2_norm_backward on the current device: fp32 partial sums of dweight and dbias.  0 if neither is wanted
+ * or a size is out of range. */
+size_t fwa2_norm_workspace_bytes(const fwa2_norm* p);
+int fwa2_norm_forward(const fwa2_norm* p);
+/* dx, dshortcut, dweight, dbias; bit-reproducible (partial sums are added in a fixed order). */
+int fwa2_norm_backward(const fwa2_norm* p);
+
+/*
+ * 8-bit form of each row of x ([rows, dim], `dtype` F16, BF16 or F32): scale = max(max |x|, 2^-100) * fp32(1 / 448)
+ * in fp32, q = x / scale rounded to e4m3 (ties to even).  q is [rows, dim] contiguous, scale [rows].  A row that holds an infinity or a NaN
+ * gets a scale that is not finite (or NaN), so that what is computed from it is not finite either.
+ */
+int fwa2_quantize_rows(const void* x, int dtype, int64_t rows, int dim, int64_t x_stride, void* q, float* scale,
+                       void* stream);
+
+/*
+ * y = act(x weight^T + bias) + residual for x [rows, in_features], weight [out_features, in_features]; products
+ * accumulated in fp32, y rounded once.  Backward, with z = x weight^T + bias (the sum before the activation) and
+ * dz = dy act'(z): dx = dz weight, dweight = dz^T x, dbias = the column sums of dz (dresidual is dy).  z is kept in
+ * `dtype`, and dz is rounded to `dtype` for the products, as it would be between two calls of a framework.
+ * With x_dtype = FWA2_E4M3 (forward only) x and weight hold e4m3 values with one fp32 scale per row of each:
+ * z = x_scale[i] weight_scale[j] (x weight^T)[i][j] + bias[j].
+ */
+typedef struct fwa2_linear {
+    uint32_t struct_bytes;  /* sizeof(fwa2_linear) as the caller compiled it */
+    uint32_t abi_version;   /* FWA2_ABI_VERSION */
+    int32_t dtype;          /* FWA2_F16 or FWA2_BF16: bias, residual, y, z and all gradients */
+    int32_t x_dtype;        /* of x and weight: `dtype` or FWA2_E4M3 */
+    int32_t activation;     /* fwa2_activation */
+    int32_t in_features;    /* 1 .. 2^24 - 1 */
+    int32_t out_features;   /* 1 .. 2^24 - 1 */
+    int32_t reserved;       /* 0 */
+    int64_t rows;           /* 1 .. 2^31 - 1 */
+
+    const void* x;          /* [rows, in_features], rows x_stride elements apart (below 2^22, as all row strides) */
+    int64_t     x_stride;
+    const void* weight;     /* [out_features, in_features] */
+    int64_t     weight_stride;
+    const void* bias;       /* [out_features] or NULL */
+    const void* residual;   /* [rows, out_features] or NULL */
+    int64_t     residual_stride;
+    const float* x_scale;       /* [rows], with FWA2_E4M3 */
+    const float* weight_scale;  /* [out_features], with FWA2_E4M3 */
+    void*       y;          /* [rows, out_features] contiguous; backward: not read */
+    void*       z;          /* [rows, out_features] contiguous.  Forward: written unless NULL.  Backward: read, needed
+                               unless the activation is NONE */
+    /* (backward) */
+    const void* dy;         /* [rows, out_features] */
+    int64_t     dy_stride;
+    void* dx;               /* [rows, in_features] contiguous, or NULL = not wanted */
+    void* dweight;          /* [out_features, in_features] contiguous, or NULL = not wanted */
+    void* dbias;            /* [out_features], or NULL = not wanted; wanted only together with dweight */
+
+    void* workspace;        /* fwa2_linear_workspace_bytes(p, backward) bytes, 256-byte aligned, uninitialised */
+    size_t workspace_bytes;
+    void* stream;           /* hipStream_t */
+} fwa2_linear;
+
+int fwa2_linear_validate(const fwa2_linear* p, int backward);
+/* Scratch of one call on the current device: partial products that are added afterwards in a fixed order and, for a
+ * backward call behind an activation, dz.  0 if none or a size is out of range. */
+size_t fwa2_linear_workspace_bytes(const fwa2_linear* p, int backward);
+int fwa2_linear_forward(const fwa2_linear* p);
+int fwa2_linear_backward(const fwa2_linear* p);
+
 #ifdef __cplusplus
 }
 #endif
