@@ -534,7 +534,8 @@ int fwa2_quantize_rows(const void* x, int dtype, int64_t rows, int dim, int64_t 
 static int check_linear_sizes(const fwa2_linear* p) {
     if (p->rows < 1 || p->rows > 0x7fffffffLL || p->in_features < 1 || p->out_features < 1)
         return fail(FWA2_ERR_INVALID_ARGUMENT, "linear: rows must be 1 .. 2^31 - 1, in_features and out_features positive");
-    if (p->in_features >= (1 << 24) || p->out_features >= (1 << 24) || !fwa2::linear_fits(p))
+    // (rows of 2^22 values: the rows of a tile stay below 2^31 bytes)
+    if (p->in_features >= (1 << 22) || p->out_features >= (1 << 22) || !fwa2::linear_fits(p))
         return fail(FWA2_ERR_UNSUPPORTED, "linear: %lld x %d x %d is too large for one launch", (long long)p->rows, p->in_features, p->out_features);
     return FWA2_OK;
 }
@@ -572,8 +573,6 @@ static int validate_linear(const fwa2_linear* p, int backward) {
         if ((rc = check_matrix("dy", p->dy, p->dy_stride, p->out_features, 2))) return rc;
         if (p->activation != FWA2_ACT_NONE) {
             if ((rc = check_ptr("z", p->z, 2))) return rc;
-            // dz has rows of out_features
-            if (p->out_features >= (1 << 22)) return fail(FWA2_ERR_UNSUPPORTED, "linear: out_features is beyond 2^22");
         }
         if (p->dx && (rc = check_ptr("dx", p->dx, 2))) return rc;
         if (p->dweight && (rc = check_ptr("dweight", p->dweight, 2))) return rc;

@@ -17,6 +17,9 @@
 // dW contracts over the rows of the batch and has few output tiles: the rows are split over workgroups, whose fp32
 // partial tiles are added in a fixed order by a second kernel.  dbias is the same contraction against ones and rides on the
 // matrix pipe of the workgroups with the first column tile.
+#include <initializer_list>
+#include <type_traits>
+
 #include "fwa2_common.hpp"
 
 // One half of this file per compile: 1 the bf16 products and the host code, 2 fp16, 3 the 8-bit products.
@@ -31,9 +34,9 @@ struct LinArgs {
     int64_t p_stride, q_stride;   // bytes between their memory rows
     int64_t nq, nk;               // extents: q rows of the output, contraction
     int np;                       // columns of the output
-    int tiles_p;
-    int64_t tiles;                // output tiles
-    int splits;                   // of the contraction
+    uint32_t tiles, tiles_p;      // output tiles, and those of a row of tiles
+    uint32_t splits;              // of the contraction
+    uint64_t by_tiles, by_tiles_p;    // ceil(2^40 / divisor): workgroup indices stay below 2^23
     int64_t k_per_split;          // a multiple of the stage
     void* out;                    // [nq, np] of the element type, contiguous
     float* part;                  // [splits, nq, np] fp32 instead, with splits > 1
@@ -57,17 +60,58 @@ template <int DT> struct LinElem { static constexpr int bytes = 2; };
 template <> struct LinElem<FWA2_E4M3> { static constexpr int bytes = 1; };
 
 // ---- activations -------------------------------------------------------------------------------------------
+// Upper tail Q(u) = 1 - Phi(u) of the normal distribution for u >= 0.  log2 Q is so smooth that a polynomial of degree 7 (a
+// minimax fit over [0, 6], weighted by (u + 0.35) Q(u), value at 0 fixed) gives Q to 8e-7 absolutely and 5e-5 relatively
+// over the fit, and falls on beyond it (6e-16 at 8, 0 from 20 on, where u is cut so that infinity meets a zero).  Eight
+// instructions and one exponential: the library's erff takes about 40, which in the epilogue of a product with few
+// contraction elements (96 -> 384) was more than everything else together (249 us of which 130 by count, 49 by memory).
+__device__ __forceinline__ float normal_tail(float u) {
+    float p = -1.1775869097618852e-06f;
+    p = __builtin_fmaf(p, u, 4.9426900659454986e-05f);
+    p = __builtin_fmaf(p, u, -0.0008448792505078018f);
+    p = __builtin_fmaf(p, u, 0.008222263306379318f);
+    p = __builtin_fmaf(p, u, -0.053498417139053345f);
+    p = __builtin_fmaf(p, u, -0.4588005840778351f);
+    p = __builtin_fmaf(p, u, -1.151161789894104f);
+    p = __builtin_fmaf(p, u, -1.0f);
+    return fast_exp2(p);
+}
+// z Phi(z) = max(z, 0) - u Q(u) with u = |z|, the maximum as (z + |z|) / 2 so that NaN and infinity pass through
+__device__ __forceinline__ float gelu_of(float z) {
+    const float u = fminf(fabsf(z), 20.f);
+    return __builtin_fmaf(0.5f, z + fabsf(z), -u * normal_tail(u));
+}
+__device__ __forceinline__ float sigmoid_of(float x) { return fast_rcp(1.f + fast_exp2(-kLog2e * x)); }
+constexpr float kTanhA = 1.5957691216057308f;       // 2 sqrt(2 / pi): z / 2 (1 + tanh(u)) = z sigmoid(2 u)
+constexpr float kTanhB = 0.07135481282553505f;      // 0.044715 times that
+
 __device__ __forceinline__ float act_of(float z, int act) {
     switch (act) {
-        case FWA2_ACT_GELU: return z * (0.5f * (1.f + erff(z * 0.70710678118654752f)));
-        case FWA2_ACT_GELU_TANH: {
-            // z sigmoid(2u) = z / 2 (1 + tanh(u))
-            const float u2 = z * (1.5957691216057308f + 0.07135481282553505f * z * z);
-            return z / (1.f + __expf(-u2));
-        }
-        case FWA2_ACT_SILU: return z / (1.f + __expf(-z));
+        case FWA2_ACT_GELU: return gelu_of(z);
+        case FWA2_ACT_GELU_TANH: return z * sigmoid_of(z * (kTanhA + kTanhB * z * z));
+        case FWA2_ACT_SILU: return z * sigmoid_of(z);
         case FWA2_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
         default: return z;
+    }
+}
+// 8 values; ACT < 0: the decision is taken here, once
+template <int ACT>
+__device__ __forceinline__ void act8(float* v, int act) {
+    if (ACT >= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_of(v[j], ACT);
+    } else if (act == FWA2_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_of(v[j], FWA2_ACT_GELU);
+    } else if (act == FWA2_ACT_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_of(v[j], FWA2_ACT_GELU_TANH);
+    } else if (act == FWA2_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_of(v[j], FWA2_ACT_SILU);
+    } else if (act == FWA2_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = act_of(v[j], FWA2_ACT_RELU);
     }
 }
 // d act / dz.  Beyond |z| = 100 every slope is 0 or 1 to fp32, and z (kept in 16 bits, possibly overflowed to infinity) must
@@ -75,15 +119,18 @@ __device__ __forceinline__ float act_of(float z, int act) {
 __device__ __forceinline__ float slope_of(float z, int act) {
     if (fabsf(z) > 100.f) z = copysignf(100.f, z);
     switch (act) {
-        case FWA2_ACT_GELU:
-            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+        case FWA2_ACT_GELU: {       // Phi(z) + z phi(z)
+            const float q = normal_tail(fminf(fabsf(z), 20.f));
+            const float phi = fast_exp2(-0.72134752044448170f * z * z) * 0.3989422804014327f;
+            return __builtin_fmaf(z, phi, z > 0.f ? 1.f - q : q);
+        }
         case FWA2_ACT_GELU_TANH: {
             const float z2 = z * z;
-            const float s = 1.f / (1.f + __expf(-z * (1.5957691216057308f + 0.07135481282553505f * z2)));
-            return s + z * s * (1.f - s) * (1.5957691216057308f + 0.21406443847660515f * z2);
+            const float s = sigmoid_of(z * (kTanhA + kTanhB * z2));
+            return s + z * s * (1.f - s) * (kTanhA + 3.f * kTanhB * z2);
         }
         case FWA2_ACT_SILU: {
-            const float s = 1.f / (1.f + __expf(-z));
+            const float s = sigmoid_of(z);
             return s * (1.f + z * (1.f - s));
         }
         case FWA2_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
@@ -104,20 +151,14 @@ __device__ __forceinline__ void tile_dma(const void* src, uint32_t lds) {
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory"); }
 
-// Chunk permutation of a memory row in LDS.  Plain rows of KB = 128 (64) bytes: two (four) rows share the 256 bytes that
-// the banks span, and an operand read serves rows {0-3, 12-15} of one chunk with rows {4-11} of its neighbour.
+// Chunk permutation of a memory row in LDS.  Plain rows of KB = 64 (128) bytes: four (two) rows share the 256 bytes that the
+// banks span, and an operand read serves rows {0-3, 12-15, 20-27} (then the other 16) of one chunk at a time.
 template <int KB>
-__device__ __forceinline__ int plain_swizzle(int row) {
-    if (KB == 128) return (row >> 1) & 7;
-    const int v = (row >> 2) & 3;
-    return ((v & 1) << 1) ^ ((v >> 1) * 3);
-}
-// Transposed rows of R columns: a read serves 8 contraction rows {0-3, 8-11} with 32 bytes each.  In units of 32 bytes.
+__device__ __forceinline__ int plain_swizzle(int row) { return KB == 64 ? (row >> 2) & 3 : (row >> 1) & 7; }
+// Transposed rows of R columns: a read serves 4 contraction rows with 64 bytes (4 chunks) each.  Rows of a multiple of 256
+// bytes all start on the same bank; of an odd multiple of 128, every second one does.
 template <int R>
-__device__ __forceinline__ int turned_swizzle(int k) {
-    if (R >= 128) return (k & 3) | (((k >> 3) & 1) << 2);
-    return ((k >> 1) & 1) | (((k >> 3) & 1) << 1);
-}
+__device__ __forceinline__ int turned_swizzle(int k) { return R % 128 == 0 ? 4 * (k & 3) : 4 * ((k >> 1) & 1); }
 
 // One operand's tile: R rows (columns, transposed) by one stage of the contraction.
 template <int DT, bool TURNED, int R, int KB, int NW, bool VEC>
@@ -130,13 +171,33 @@ struct Operand {
     static_assert(NI * 1024 * NW == BYTES, "whole copies");
     static constexpr int CE = 16 / EB;                      // elements of a chunk
 
+    // LDS rows of a copy; 0: copies end inside rows (192 transposed columns: 24 chunks a row)
+    static constexpr int RPC = 64 % CPR == 0 ? 64 / CPR : 0;
+    // the swizzles look at bits 0 .. 3 of a row, and the copies of a wavefront lie a multiple of that apart
+    static_assert(RPC == 0 || NW * RPC % (TURNED ? 4 : 16) == 0, "");
+
     const char* base;       // uniform: first row (column) of the tile, first contraction element of the split
     int64_t stride;
     int64_t step;           // bytes from stage to stage
-    uint32_t off[VEC ? NI : 1];
+    uint32_t off[NI];       // of this lane's chunk of each copy
     int rows;               // rows (columns) of the tile inside the matrix
+    int row0, chunk0;       // of this lane's part of copy 0 (place)
     int wave, lane;
 
+    static __device__ __forceinline__ int swizzled(int row, int c) { return c ^ (TURNED ? turned_swizzle<R>(row) : plain_swizzle<KB>(row)); }
+    // LDS row of this lane's part of copy i, and the memory chunk that belongs there
+    __device__ __forceinline__ void place(int i, int& row, int& chunk) const {
+        if (RPC > 0) {
+            row = row0 + i * NW * RPC;
+            chunk = chunk0;
+        } else {
+            const int ci = (i * NW + wave) * 64 + lane;
+            row = ci / CPR;
+            chunk = swizzled(row, ci - row * CPR);
+        }
+    }
+
+    // Rows (columns) beyond the matrix repeat the last ones: what they produce is not stored.
     __device__ __forceinline__ void init(const char* ptr, int64_t str, int64_t first, int64_t extent, int64_t k0, int w, int l) {
         stride = str;
         wave = w;
@@ -151,26 +212,15 @@ struct Operand {
             step = KB;
         }
         base = reinterpret_cast<const char*>(uniform_pointer(base));
-        if (VEC) {
+        row0 = wave * RPC + lane / CPR;
+        chunk0 = swizzled(row0, lane % CPR);
 #pragma unroll
-            for (int i = 0; i < NI; i++) {
-                int row, c;
-                place(i, row, c);
-                off[i] = offset(row, c);
-            }
+        for (int i = 0; i < NI; i++) {
+            int r, chunk;
+            place(i, r, chunk);
+            if (TURNED) off[i] = (uint32_t)r * (uint32_t)stride + (uint32_t)(chunk * CE < rows ? chunk * 16 : rows * EB - 16);
+            else off[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)stride + (uint32_t)chunk * 16;
         }
-    }
-    // LDS row of this lane's part of copy i, and the memory chunk that belongs there
-    __device__ __forceinline__ void place(int i, int& row, int& c) const {
-        const int ci = (i * NW + wave) * 64 + lane;
-        row = ci / CPR;
-        c = ci % CPR;
-        c ^= TURNED ? 2 * turned_swizzle<R>(row) : plain_swizzle<KB>(row);
-    }
-    // Rows (columns) beyond the matrix repeat the last ones: what they produce is not stored.
-    __device__ __forceinline__ uint32_t offset(int row, int c) const {
-        if (TURNED) return (uint32_t)row * (uint32_t)stride + (uint32_t)(c * CE < rows ? c * 16 : rows * EB - 16);
-        return (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)stride + (uint32_t)c * 16;
     }
     // Ask for stage kt, of which `left` contraction elements are inside the matrix.
     __device__ __forceinline__ void issue(int64_t kt, int left, char* lds) const {
@@ -182,10 +232,10 @@ struct Operand {
         } else {
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                int row, c;
-                place(i, row, c);
-                const bool in = TURNED ? row < left : c * CE < left;
-                const void* src = in ? (const void*)(at + offset(row, c)) : (const void*)k_zeros;
+                int row, chunk;
+                place(i, row, chunk);
+                const bool in = TURNED ? row < left : chunk * CE < left;
+                const void* src = in ? (const void*)(at + off[i]) : (const void*)k_zeros;
                 tile_dma(src, dst + i * NW * 1024);
             }
         }
@@ -195,16 +245,16 @@ struct Operand {
         const char* at = base + kt * step;
 #pragma unroll
         for (int i = 0; i < NI; i++) {
-            int row, c;
-            place(i, row, c);
+            int at_row, chunk;
+            place(i, at_row, chunk);
             int n;              // elements of the chunk inside the matrix
             const char* src;
             if (TURNED) {
-                n = row < left ? rows - c * CE : 0;
-                src = at + (int64_t)row * stride + c * 16;
+                n = at_row < left ? rows - chunk * CE : 0;
+                src = at + (int64_t)at_row * stride + chunk * 16;
             } else {
-                n = left - c * CE;
-                src = at + (int64_t)(row < rows ? row : rows - 1) * stride + c * 16;
+                n = left - chunk * CE;
+                src = at + (int64_t)(at_row < rows ? at_row : rows - 1) * stride + chunk * 16;
             }
             r[i] = u32x4{0, 0, 0, 0};
             if (n >= CE) {
@@ -229,137 +279,126 @@ struct Operand {
     }
 };
 
-// MFMA operands of 16 rows out of a staged tile.
-template <int DT> struct Frag {
+// MFMA operands of 32 rows out of a staged tile: lane (row = lane % 32, half = lane / 32).  Which contraction elements a lane
+// holds does not matter as long as both operands agree.
+template <int DT> struct Frag {             // v_mfma_f32_32x32x16
     typedef typename Elem<DT>::V8 V;
-    static constexpr int K = 32;
-    static __device__ __forceinline__ V plain(const char* tile, int row, int swz, int g, int kk, int kb) {
-        return *reinterpret_cast<const V*>(tile + row * kb + (((kk * 4 + g) ^ swz) * 16));
+    static constexpr int BYTES = 32;        // of a row per product
+    template <int KB>
+    static __device__ __forceinline__ V plain(const char* tile, int row, int swz, int half, int s) {
+        return *reinterpret_cast<const V*>(tile + row * KB + (((2 * s + half) ^ swz) * 16));
     }
-    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) { return Elem<DT>::mfma16(a, b, c); }
+    template <int R>
+    static __device__ __forceinline__ V turned(const char* tile, int t32, int lane, int s) {
+        const int i = lane & 15, g = lane >> 4;
+        const int k = 16 * s + 8 * (g >> 1) + (i >> 2);
+        const int chunk = (4 * t32 + 2 * (g & 1) + ((i & 3) >> 1)) ^ turned_swizzle<R>(k);
+        typedef typename Elem<DT>::E E;
+        const E* lo = reinterpret_cast<const E*>(tile + k * R * 2 + chunk * 16 + (i & 1) * 8);
+        return lds_tr8<DT>(lo, lo + 4 * R);
+    }
+    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) { return Elem<DT>::mfma32(a, b, c); }
 };
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-template <> struct Frag<FWA2_E4M3> {
+template <> struct Frag<FWA2_E4M3> {        // v_mfma_f32_32x32x64
     typedef i32x8 V;
-    static constexpr int K = 128;
-    // A lane takes chunks g and g + 4 of its row: which contraction elements a lane holds does not matter as long as both
-    // operands agree, and these two keep the banks apart.
-    static __device__ __forceinline__ V plain(const char* tile, int row, int swz, int g, int kk, int kb) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(tile + row * kb + ((g ^ swz) * 16));
-        const u32x4 b = *reinterpret_cast<const u32x4*>(tile + row * kb + (((g + 4) ^ swz) * 16));
+    static constexpr int BYTES = 64;
+    template <int KB>
+    static __device__ __forceinline__ V plain(const char* tile, int row, int swz, int half, int s) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(tile + row * KB + (((4 * s + half) ^ swz) * 16));
+        const u32x4 b = *reinterpret_cast<const u32x4*>(tile + row * KB + (((4 * s + 2 + half) ^ swz) * 16));
         V v;
 #pragma unroll
         for (int i = 0; i < 4; i++) { v[i] = (int)a[i]; v[4 + i] = (int)b[i]; }
         return v;
     }
+    template <int R>
+    static __device__ __forceinline__ V turned(const char*, int, int, int) { return V{}; }
     // The 8-bit unit adds products in groups of 8 contraction elements aligned to the group's largest and drops what lies
-    // below 2^-13 of that (measured, for this form as for the 32-element one); the groups are added in fp32.  Against the
-    // 2^-4 half steps of the operands that is nothing, and the alternative, converting the tiles to 16 bits for the
-    // exact products of the other unit, halves the matrix rate.
+    // below 2^-13 of that (measured, for the 16x16x128 form as for the 16x16x32 one); the groups are added in fp32.  Against
+    // the 2^-4 half steps of the operands that is nothing, and the alternative, converting the tiles to 16 bits for
+    // the exact products of the other unit, halves the matrix rate.
     // 0x7f: a block scale of 2^0 in every byte
-    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    static __device__ __forceinline__ f32x16 mfma(V a, V b, f32x16 c) {
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
     }
 };
-template <int DT, int R>
-__device__ __forceinline__ typename Elem<DT>::V8 frag_turned(const char* tile, int t16, int l16, int g, int kk) {
-    const int k = kk * 32 + 8 * g + (l16 >> 2);
-    const int at = k * R * 2 + ((t16 ^ turned_swizzle<R>(k)) * 32) + (l16 & 3) * 8;
-    typedef typename Elem<DT>::E E;
-    const E* lo = reinterpret_cast<const E*>(tile + at);
-    return lds_tr8<DT>(lo, lo + 4 * R);
-}
 
 // Which tile a workgroup computes.  Workgroups go to the 8 XCDs in turn, each with an L2 of its own: consecutive tiles are
 // given to one XCD, column tiles first, so that the tiles that share a block of Q rows meet in one L2.
-__device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t total) {
-    const int64_t per = (total + 7) / 8;
+__device__ __forceinline__ uint32_t tile_of_block(uint32_t block, uint32_t total) {
+    const uint32_t per = (total + 7) / 8;
     return (block & 7) * per + (block >> 3);
 }
+// n / d for n < 2^23, d < 2^17, from ceil(2^40 / d): the excess of the quotient is below n d / 2^40 / d < 1 / d
+__device__ __forceinline__ uint32_t divide(uint32_t n, uint64_t by) { return (uint32_t)((n * by) >> 40); }
 
-template <class OT>
-__device__ __forceinline__ void epilogue8(const LinArgs& a, float* v, const float* bias, int64_t q, int p, int n) {
-    typedef OT V8 __attribute__((ext_vector_type(8)));
+// The values as fp32 numbers of their own: what follows must not be folded into the arithmetic before it.  (The compiler
+// turns a multiply-add and its conversion to fp16 into one instruction with one rounding in some forms of the epilogue and
+// not in others; a call with and one without gradients would then differ in the last bit.)
+__device__ __forceinline__ void settle8(float* v) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] += bias[j];
-    OT* z = reinterpret_cast<OT*>(a.z);
-    OT* out = reinterpret_cast<OT*>(a.out);
-    const int64_t at = q * a.np + p;
-    if (a.out_vec) {        // np is a multiple of 8: the chunk is inside or outside as a whole
-        if (z != nullptr) {
-            V8 t;
+    for (int j = 0; j < 8; j++) asm("" : "+v"(v[j]));
+}
+
+// N bias values from column p on.  Columns beyond the last repeat it (their results are not stored): no branch, and with
+// whole groups (np a multiple of 8, bias aligned) one load.
+template <class OT, int N>
+__device__ __forceinline__ void load_bias(const LinArgs& a, int p, float* b) {
+    typedef OT VN __attribute__((ext_vector_type(N)));
+    const OT* src = reinterpret_cast<const OT*>(a.bias);
+    if (a.out_vec) {
+        const VN v = *reinterpret_cast<const VN*>(src + min(p, a.np - N));
 #pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
-            *reinterpret_cast<V8*>(z + at) = t;
-        }
-        if (a.act != FWA2_ACT_NONE)
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = act_of(v[j], a.act);
-        if (a.residual != nullptr) {
-            const V8 r = *reinterpret_cast<const V8*>(reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + p);
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] += (float)r[j];
-        }
-        V8 t;
-#pragma unroll
-        for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
-        *reinterpret_cast<V8*>(out + at) = t;
+        for (int j = 0; j < N; j++) b[j] = (float)v[j];
     } else {
-        const OT* r = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (j >= n) continue;
-            if (z != nullptr) z[at + j] = (OT)v[j];
-            float y = act_of(v[j], a.act);
-            if (a.residual != nullptr) y += (float)r[p + j];
-            out[at + j] = (OT)y;
-        }
-    }
-}
-template <class OT>
-__device__ __forceinline__ void bias8(const LinArgs& a, int p, float* b) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) b[j] = a.bias != nullptr && p + j < a.np ? (float)reinterpret_cast<const OT*>(a.bias)[p + j] : 0.f;
-}
-
-// Two accumulator tiles of 16 output columns become 8 consecutive columns per lane: the lanes of rows 1 and 3 of the first
-// change places with those of rows 0 and 2 of the second.  Column of the lane's first value within the 32:
-__device__ __forceinline__ int pair_column(int g) { return ((g & 1) << 4) | ((g >> 1) << 3); }
-__device__ __forceinline__ void pair_swap(f32x4 a, f32x4 b, float* v) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[r]), __float_as_uint(b[r]), false, false);
-        v[r] = __uint_as_float(s[0]);
-        v[4 + r] = __uint_as_float(s[1]);
+        for (int j = 0; j < N; j++) b[j] = (float)src[min(p + j, a.np - 1)];
     }
 }
 
-template <int DT, bool PT, bool QT, int BP, int BQ, int WP, int WQ, int KB, int STAGES, bool VEC>
-__global__ void __launch_bounds__(64 * WP * WQ) linear_kernel(const LinArgs a) {
+// Where 16-byte chunk c of row q of a wavefront's 32 x TP block of results lies in LDS: rows of TP floats, chunks permuted so
+// that neither the writes (one chunk of 16 rows at a time) nor the reads (whole rows) pile up on a bank.
+template <int TP>
+__device__ __forceinline__ int result_chunk(int q, int c) {
+    const int x = TP == 32 ? (q >> 1) & 7 : TP % 64 == 0 ? q & 15 : q & 7;
+    return q * (TP / 4) + (c ^ x);
+}
+
+// ACT: the activation, or -1 where it is decided at run time.  WAVES: wavefronts per SIMD the registers are limited for.
+template <int DT, bool PT, bool QT, int BP, int BQ, int WP, int WQ, int KB, int STAGES, bool VEC, int ACT, int WAVES>
+__global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinArgs a) {
     constexpr int NW = WP * WQ;
     constexpr int TP = BP / WP, TQ = BQ / WQ;       // a wavefront's part of the tile
-    constexpr int FP = TP / 16, FQ = TQ / 16;
-    static_assert(TP % 32 == 0 && TQ % 16 == 0, "");
+    constexpr int FP = TP / 32, FQ = TQ / 32;
+    static_assert(TP % 32 == 0 && TQ % 32 == 0 && STAGES >= 2, "");
     typedef Operand<DT, PT, BP, KB, NW, VEC> OP;
     typedef Operand<DT, QT, BQ, KB, NW, VEC> OQ;
+    typedef Frag<DT> F;
+    typedef typename F::V FV;
     constexpr int KE = OP::KE;
-    constexpr int KSTEPS = KE / Frag<DT>::K;
+    constexpr int STEPS = KB / F::BYTES;         // products of a stage and 32 x 32 tile
     constexpr int STAGE = OP::BYTES + OQ::BYTES;
+    constexpr int COPIES = OP::NI + OQ::NI;         // outstanding memory operations of a stage, per wavefront
     constexpr bool DB = PT && QT;
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE];
+    typedef typename Elem<DT == FWA2_E4M3 ? FWA2_F16 : DT>::E E16;
+    constexpr int RESULTS = NW * 32 * TP * 4;       // the results pass through the same memory afterwards
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * STAGE > RESULTS ? STAGES * STAGE : RESULTS];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % WP, wq = wave / WP;
-    const int l16 = lane & 15, g = lane >> 4;
+    const int l32 = lane & 31, half = lane >> 5;
 
-    const int64_t total = a.tiles * a.splits;
-    const int64_t t = tile_of_block(blockIdx.x, total);
+    const uint32_t total = a.tiles * a.splits;
+    const uint32_t t = tile_of_block(blockIdx.x, total);
     if (t >= total) return;
-    const int64_t tile = t / a.splits;
-    const int split = (int)(t - tile * a.splits);
-    const int64_t q0 = (tile / a.tiles_p) * BQ;
-    const int p0 = (int)(tile % a.tiles_p) * BP;
+    // split by split: the tiles that read the same stretch of the contraction run side by side
+    const uint32_t split = a.splits > 1 ? divide(t, a.by_tiles) : 0;
+    const uint32_t tile = t - split * a.tiles;
+    const uint32_t tile_q = divide(tile, a.by_tiles_p);
+    const int64_t q0 = (int64_t)tile_q * BQ;
+    const int p0 = (int)(tile - tile_q * a.tiles_p) * BP;
     const int64_t k0 = split * a.k_per_split;
     const int64_t k1 = k0 + a.k_per_split < a.nk ? k0 + a.k_per_split : a.nk;
     const int64_t len = k1 - k0;
@@ -371,74 +410,94 @@ __global__ void __launch_bounds__(64 * WP * WQ) linear_kernel(const LinArgs a) {
     P.init(a.p, a.p_stride, p0, a.np, k0, wave, lane);
     Q.init(a.q, a.q_stride, q0, a.nq, k0, wave, lane);
 
-    f32x4 acc[FQ][FP];
+    f32x16 acc[FQ][FP];
 #pragma unroll
     for (int i = 0; i < FQ; i++)
 #pragma unroll
-        for (int j = 0; j < FP; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f32x4 accb[DB ? FQ : 1];
+        for (int j = 0; j < FP; j++) acc[i][j] = f32x16{};
+    float row_sums[DB ? FQ : 1];
 #pragma unroll
-    for (int i = 0; i < (DB ? FQ : 1); i++) accb[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < (DB ? FQ : 1); i++) row_sums[i] = 0.f;
     const bool sum_rows = DB && a.db != nullptr && p0 == 0 && wp == 0;
 
-    auto compute = [&](const char* buf, int left) __attribute__((always_inline)) {
-        const char* tp = buf;
-        const char* tq = buf + OP::BYTES;
-        const int swz = plain_swizzle<KB>(l16);
+    const int swz = plain_swizzle<KB>(l32);
+    auto load_p = [&](const char* buf, int s, int j) __attribute__((always_inline)) -> FV {
+        if constexpr (PT) return F::template turned<BP>(buf, wp * FP + j, lane, s);
+        else return F::template plain<KB>(buf, wp * TP + 32 * j + l32, swz, half, s);
+    };
+    auto load_q = [&](const char* buf, int s, int i) __attribute__((always_inline)) -> FV {
+        if constexpr (QT) return F::template turned<BQ>(buf + OP::BYTES, wq * FQ + i, lane, s);
+        else return F::template plain<KB>(buf + OP::BYTES, wq * TQ + 32 * i + l32, swz, half, s);
+    };
+    FV fp[FP], fq[FQ];
+    auto load = [&](const char* buf, int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < KSTEPS; kk++) {
-            if (kk * Frag<DT>::K >= left) break;
-            typename Frag<DT>::V fp[FP], fq[FQ];
+        for (int i = 0; i < FQ; i++) fq[i] = load_q(buf, s, i);
 #pragma unroll
-            for (int j = 0; j < FP; j++) {
-                if constexpr (PT) fp[j] = frag_turned<DT, BP>(tp, wp * FP + j, l16, g, kk);
-                else fp[j] = Frag<DT>::plain(tp, wp * TP + 16 * j + l16, swz, g, kk, KB);
-            }
+        for (int j = 0; j < FP; j++) fp[j] = load_p(buf, s, j);
+    };
+    auto add_rows = [&]() __attribute__((always_inline)) {
+        if constexpr (DB) {
+            if (sum_rows) {
 #pragma unroll
-            for (int i = 0; i < FQ; i++) {
-                if constexpr (QT) fq[i] = frag_turned<DT, BQ>(tq, wq * FQ + i, l16, g, kk);
-                else fq[i] = Frag<DT>::plain(tq, wq * TQ + 16 * i + l16, swz, g, kk, KB);
-            }
+                for (int i = 0; i < FQ; i++)
 #pragma unroll
-            for (int i = 0; i < FQ; i++)
-#pragma unroll
-                for (int j = 0; j < FP; j++) acc[i][j] = Frag<DT>::mfma(fp[j], fq[i], acc[i][j]);
-            if constexpr (DB) {
-                if (sum_rows) {
-                    typename Frag<DT>::V ones;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) ones[j] = (typename Elem<DT>::E)1.f;
-#pragma unroll
-                    for (int i = 0; i < FQ; i++) accb[i] = Frag<DT>::mfma(ones, fq[i], accb[i]);
-                }
+                    for (int e = 0; e < 8; e++) row_sums[DB ? i : 0] += (float)fq[i][e];
             }
         }
     };
+    auto multiply = [&]() __attribute__((always_inline)) {
+        add_rows();
+#pragma unroll
+        for (int j = 0; j < FP; j++)
+#pragma unroll
+            for (int i = 0; i < FQ; i++) acc[i][j] = F::mfma(fp[j], fq[i], acc[i][j]);
+    };
+    // The products of the operands in registers, each P operand replaced by step s of `buf` as soon as it has been used: the
+    // LDS reads of a step run under the matrix work of the one before it.
+    auto multiply_and_load = [&](const char* buf, int s) __attribute__((always_inline)) {
+        add_rows();
+        FV qn[FQ];
+#pragma unroll
+        for (int i = 0; i < FQ; i++) qn[i] = load_q(buf, s, i);
+#pragma unroll
+        for (int j = 0; j < FP; j++) {
+#pragma unroll
+            for (int i = 0; i < FQ; i++) acc[i][j] = F::mfma(fp[j], fq[i], acc[i][j]);
+            fp[j] = load_p(buf, s, j);
+        }
+#pragma unroll
+        for (int i = 0; i < FQ; i++) fq[i] = qn[i];
+    };
 
     if constexpr (VEC) {
-        static_assert(STAGES >= 2, "");
+        auto issue = [&](int64_t kt, char* buf) __attribute__((always_inline)) {
+            P.issue(kt, left_of(kt), buf);
+            Q.issue(kt, left_of(kt), buf + OP::BYTES);
+        };
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; s++) {
-            if (s < nkt) {
-                P.issue(s, left_of(s), lds + s * STAGE);
-                Q.issue(s, left_of(s), lds + s * STAGE + OP::BYTES);
-            }
-        }
-        int cur = 0, nxt = STAGES - 1;
-        for (int64_t kt = 0; kt < nkt; kt++) {
-            // stage kt has landed when at most the copies of the later stages are still out
-            if (kt + STAGES - 1 <= nkt) wait_vm<(STAGES - 2) * (OP::NI + OQ::NI)>();
+        for (int s = 0; s < STAGES; s++)
+            if (s < nkt) issue(s, lds + s * STAGE);
+        if (nkt >= STAGES) wait_vm<(STAGES - 1) * COPIES>();
+        else wait_vm<0>();
+        lds_barrier();
+        load(lds, 0);
+        char* cur = lds;
+        for (int64_t kt = 0; kt + 1 < nkt; kt++) {
+            char* next = cur + STAGE == lds + STAGES * STAGE ? lds : cur + STAGE;
+#pragma unroll
+            for (int s = 1; s < STEPS; s++) multiply_and_load(cur, s);
+            // stage kt + 1 has landed when at most the copies of the later stages are still out ...
+            if (kt + STAGES <= nkt) wait_vm<(STAGES - 2) * COPIES>();
             else wait_vm<0>();
-            lds_barrier();      // ... for every wavefront, and all have read the stage that the next copies overwrite
-            const int64_t kn = kt + STAGES - 1;
-            if (kn < nkt) {
-                P.issue(kn, left_of(kn), lds + nxt * STAGE);
-                Q.issue(kn, left_of(kn), lds + nxt * STAGE + OP::BYTES);
-            }
-            compute(lds + cur * STAGE, left_of(kt));
-            cur = cur + 1 == STAGES ? 0 : cur + 1;
-            nxt = nxt + 1 == STAGES ? 0 : nxt + 1;
+            lds_barrier();      // ... for every wavefront, and all hold the rest of stage kt in registers: its place is free
+            if (kt + STAGES < nkt) issue(kt + STAGES, cur);
+            multiply_and_load(next, 0);
+            cur = next;
         }
+#pragma unroll
+        for (int s = 1; s < STEPS; s++) multiply_and_load(cur, s);
+        multiply();
     } else {
         u32x4 rp[OP::NI], rq[OQ::NI];
         P.fetch(0, left_of(0), rp);
@@ -452,70 +511,213 @@ __global__ void __launch_bounds__(64 * WP * WQ) linear_kernel(const LinArgs a) {
                 P.fetch(kt + 1, left_of(kt + 1), rp);
                 Q.fetch(kt + 1, left_of(kt + 1), rq);
             }
-            compute(buf, left_of(kt));
+            load(buf, 0);
+#pragma unroll
+            for (int s = 1; s < STEPS; s++) multiply_and_load(buf, s);
+            multiply();
         }
     }
 
-    const int64_t qw = q0 + wq * TQ + l16;
-    const int pw = p0 + wp * TP;
-    if (a.splits > 1) {
-        float* out = a.part + (int64_t)split * a.nq * a.np;
+    if constexpr (DB) {
+        if (sum_rows) {
 #pragma unroll
-        for (int i = 0; i < FQ; i++) {
-            const int64_t q = qw + 16 * i;
-            if (q >= a.nq) continue;
-#pragma unroll
-            for (int j = 0; j < FP; j++) {
-                const int p = pw + 16 * j + 4 * g;
-                float* o = out + q * a.np + p;
-                if (a.np % 4 == 0) {
-                    if (p < a.np) *reinterpret_cast<f32x4*>(o) = acc[i][j];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (p + r < a.np) o[r] = acc[i][j][r];
+            for (int i = 0; i < FQ; i++) {
+                const float t = xor32_add(row_sums[DB ? i : 0]);
+                const int64_t q = q0 + wq * TQ + 32 * i + l32;
+                if (half == 0 && q < a.nq) {
+                    if (a.splits > 1) a.part_db[(int64_t)split * a.nq + q] = t;
+                    else reinterpret_cast<E16*>(a.db)[q] = (E16)t;
                 }
             }
-            if (DB && sum_rows && g == 0) a.part_db[split * a.nq + q] = accb[DB ? i : 0][0];
+        }
+    }
+    // The accumulators hold 4 consecutive columns of 32 different rows: written like that, every store would touch 32 rows
+    // with 32 bytes each.  They change hands through LDS instead (each wavefront its own part, 32 rows at a time), so that
+    // TP / 8 neighbouring lanes hold whole stretches of a row, and residual, z and result move in full cache lines.
+    lds_barrier();          // nobody reads operands any more
+    char* mine = lds + wave * 32 * TP * 4;
+    constexpr int LPR = TP / 8;             // lanes of a row
+    constexpr int RPI = 64 / LPR;           // rows per instruction (TP = 96: 5, and four lanes idle)
+    const int rl = lane / LPR, cl = lane - rl * LPR;
+    const int p = p0 + wp * TP + 8 * cl;
+    const bool inside = rl < RPI && p < a.np;
+    const int64_t qw = q0 + wq * TQ;        // uniform: first row of this wavefront
+    auto put = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FP; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const f32x4 v = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+                *reinterpret_cast<f32x4*>(mine + 16 * result_chunk<TP>(l32, 8 * j + 2 * r + half)) = v;
+            }
+        asm volatile("" ::: "memory");      // a wavefront's LDS accesses stay in order
+    };
+    auto get = [&](int row, float* v) __attribute__((always_inline)) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl + 1));
+#pragma unroll
+        for (int e = 0; e < 4; e++) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+    };
+    // Is row r0 + rl of the 32 this lane's business?  (q: the uniform part of its index in the output)
+    auto mine_row = [&](int r0, int64_t q) __attribute__((always_inline)) {
+        return inside && (32 % RPI == 0 || r0 + rl < 32) && q + rl < a.nq;
+    };
+    // uniform row pointers and a 32-bit offset per lane: no 64-bit address arithmetic on the vector unit
+    const uint32_t at = (uint32_t)rl * (uint32_t)a.np + (uint32_t)p;
+    if (a.splits > 1) {
+        float* out = a.part + (int64_t)split * a.nq * a.np;
+        const bool whole = a.np % 8 == 0;
+#pragma unroll
+        for (int i = 0; i < FQ; i++) {
+            put(i);
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += RPI) {
+                const int64_t q = qw + 32 * i + r0;
+                if (!mine_row(r0, q)) continue;
+                float v[8];
+                get(r0 + rl, v);
+                float* o = out + q * a.np + at;
+                if (whole) {
+                    *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+                    *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (p + e < a.np) o[e] = v[e];
+                }
+            }
+            asm volatile("" ::: "memory");
         }
         return;
     }
     auto finish = [&](auto tag) __attribute__((always_inline)) {
         typedef decltype(tag) OT;
+        typedef OT V8 __attribute__((ext_vector_type(8)));
+        constexpr int NR = (32 + RPI - 1) / RPI;
+        float bias[8], ps[8];
 #pragma unroll
-        for (int u = 0; u < FP / 2; u++) {
-            const int p = pw + 32 * u + pair_column(g);
-            float bias[8], ps[8];
-            bias8<OT>(a, p, bias);
+        for (int e = 0; e < 8; e++) bias[e] = 0.f;
+        if (a.bias != nullptr) load_bias<OT, 8>(a, p, bias);
+        if constexpr (DT == FWA2_E4M3) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) ps[e] = a.p_scale[min(p + e, a.np - 1)];
+        }
+        // bias, and before it the scales of an 8-bit product
+        auto scaled = [&](float* v, int64_t q) __attribute__((always_inline)) {
             if constexpr (DT == FWA2_E4M3) {
+                const float qs = a.q_scale[q];
 #pragma unroll
-                for (int j = 0; j < 8; j++) ps[j] = p + j < a.np ? a.p_scale[p + j] : 0.f;
+                for (int e = 0; e < 8; e++) v[e] = v[e] * (qs * ps[e]) + bias[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] += bias[e];
             }
+        };
+        const uint32_t res_at = (uint32_t)rl * (uint32_t)(a.residual_stride / 2) + (uint32_t)p;
+        if (a.out_vec) {        // np is a multiple of 8: a lane's 8 columns are inside or outside together
+            // Buffer accesses: rows beyond the last lie outside the buffer's size, lanes outside the columns are sent there,
+            // and the hardware drops such stores and returns zeros for such loads; no branches, and all rows in one
+            // stretch of code.  A wavefront's rows span less than 2^31 bytes (row strides are below 2^22 elements).
+            const int rows = a.nq - qw < TQ ? (int)(a.nq - qw) : TQ;
+            const bool any = rows > 0;
+            auto buffer = [&](const void* base, int64_t row_bytes) __attribute__((always_inline)) {
+                return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(uniform_pointer(reinterpret_cast<const char*>(base) + qw * row_bytes)), 0,
+                                                         any ? (int)(rows * row_bytes) : 0, 0x00027000);
+            };
+            const auto out_rows = buffer(a.out, (int64_t)a.np * 2);
+            const uint32_t out_at = inside ? at * 2 : 0x80000000u, out_step = (uint32_t)a.np * 2;
+            const uint32_t from = inside ? res_at * 2 : 0x80000000u, res_step = (uint32_t)a.residual_stride;
+            auto body = [&](auto has_residual, auto has_z) __attribute__((always_inline)) {
+                const auto res_rows = buffer(a.residual, has_residual ? a.residual_stride : 0);
+                const auto z_rows = buffer(a.z, has_z ? (int64_t)a.np * 2 : 0);
+#pragma unroll
+                for (int i = 0; i < FQ; i++) {
+                    u32x4 res[NR];
+                    if (has_residual) {
+#pragma unroll
+                        for (int k = 0; k < NR; k++)
+                            res[k] = __builtin_amdgcn_raw_buffer_load_b128(res_rows, from + (32 * i + k * RPI) * res_step, 0, 0);
+                    }
+                    put(i);
+#pragma unroll
+                    for (int k = 0; k < NR; k++) {
+                        const uint32_t skip = 32 % RPI != 0 && k * RPI + rl >= 32 ? 0x80000000u : 0u;
+                        float v[8];
+                        get(32 % RPI == 0 ? k * RPI + rl : min(k * RPI + rl, 31), v);
+                        scaled(v, any ? qw + min(32 * i + k * RPI + rl, rows - 1) : 0);
+                        settle8(v);
+                        V8 t;
+                        if (has_z) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), z_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, 0);
+                        }
+                        act8<ACT>(v, a.act);
+                        settle8(v);
+                        if (has_residual) {
+                            const V8 r = __builtin_bit_cast(V8, res[k]);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) v[j] += (float)r[j];
+                        }
+                        settle8(v);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), out_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, 0);
+                    }
+                    asm volatile("" ::: "memory");
+                }
+            };
+            const std::true_type yes;
+            const std::false_type no;
+            if (a.residual != nullptr) {
+                if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(yes, yes);
+                else body(yes, no);
+            } else {
+                if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(no, yes);
+                else body(no, no);
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < FQ; i++) {
-                const int64_t q = qw + 16 * i;
-                float v[8];
-                pair_swap(acc[i][2 * u], acc[i][2 * u + 1], v);     // exchanged by all lanes, stored by those inside
-                if (q >= a.nq || p >= a.np) continue;
-                if constexpr (DT == FWA2_E4M3) {
-                    const float qs = a.q_scale[q];
+                put(i);
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += RPI) {
+                    const int64_t q = qw + 32 * i + r0;
+                    if (!mine_row(r0, q)) continue;
+                    float v[8];
+                    get(r0 + rl, v);
+                    scaled(v, q + rl);
+                    settle8(v);
+                    const int n = a.np - p;
+                    OT* out = reinterpret_cast<OT*>(a.out) + q * a.np + at;
+                    OT* z = reinterpret_cast<OT*>(a.z) + q * a.np + at;
+                    if (a.z != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] *= qs * ps[j];
+                        for (int j = 0; j < 8; j++)
+                            if (j < n) z[j] = (OT)v[j];
+                    }
+                    act8<ACT>(v, a.act);
+                    settle8(v);
+                    if (a.residual != nullptr) {
+                        const OT* res = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + res_at;
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (j < n) v[j] += (float)res[j];
+                    }
+                    settle8(v);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (j < n) out[j] = (OT)v[j];
                 }
-                epilogue8<OT>(a, v, bias, q, p, a.np - p);
+                asm volatile("" ::: "memory");
             }
-        }
-        if (DB && sum_rows && g == 0) {
-#pragma unroll
-            for (int i = 0; i < FQ; i++)
-                if (qw + 16 * i < a.nq) reinterpret_cast<OT*>(a.db)[qw + 16 * i] = (OT)accb[DB ? i : 0][0];
         }
     };
     if constexpr (DT == FWA2_E4M3) {
         if (a.out_bf16) finish((__bf16)0.f);
         else finish((_Float16)0.f);
     } else {
-        finish((typename Elem<DT == FWA2_E4M3 ? FWA2_F16 : DT>::E)0.f);
+        finish((E16)0.f);
     }
 }
 
@@ -588,49 +790,134 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t 
 #endif
 
 // ---- launch ---------------------------------------------------------------------------------------------------
-// Sizes of a product: q rows, p columns, contraction.
+// The tile a product runs on, and how its contraction is split.
+enum Tile { T64, T128S, T128, T192P, T192Q, T192, T256 };
+struct TileShape {
+    int bp, bq, kb, per_cu;     // columns, rows, bytes of the contraction per stage, resident workgroups of a CU
+};
+static constexpr TileShape kTiles[] = {
+    {64, 64, 64, 4},      // T64:    too few output tiles of any other size to fill the chip
+    {128, 128, 64, 4},    // T128S:  short contractions: loads and stores bound the call, many workgroups hide each other's
+    {128, 128, 128, 2},   // T128
+    {192, 128, 128, 2},   // T192P:  column counts that waste less of 192 than of 128 (and equal ones: fewer operand reads)
+    {128, 192, 128, 2},   // T192Q:  the same for the rows; weight gradients only, as is
+    {192, 192, 128, 1},   // T192:   both
+    {256, 256, 128, 1},   // T256:   large products, 8 wavefronts: LDS reads per product fall with the tile's edge
+};
 struct LinPlan {
-    int bp, bq, ke;
+    Tile tile;
     int splits;
     int64_t k_per_split, tiles;
     int tiles_p;
 };
 
-// Tiles of 128 x 128 when they fill the chip, of 64 x 64 otherwise.
+// The rule, with what it was measured on (MI355X, us, bf16; rows x contraction -> columns):
+//   262144 x   96 ->  384 gelu       T128S  62, T128  94, T192P 106, T256 115, T64  94
+//    65536 x  192 ->  768 gelu, z    T128S  47, T128  50, T192P  54, T256  54, T64  70
+//    16384 x  384 -> 1536 gelu, z    T128S  40, T128  38, T192P  39, T256  44, T64  55
+//    65536 x  768 ->  192 residual   T128S  39, T128  33, T192P  26, T256  32, T64  57
+//     4096 x  768 -> 1536 gelu, z    T128S  23, T128  20, T192P  20, T256  30, T64  29
+//     2048 x 1024 -> 1024 gelu       T128S  16, T128  15, T192P  19, T256  31, T64  14
+//     8192 x 4096 -> 4096 residual   T128S 375, T128 291, T192P 283, T256 228, T64 665
+// weight gradients (rows of dW x rows of the batch -> columns of dW), splits chosen as below:
+//      384 x 262144 ->  96           T128  49, T192Q 39, T192P 64, T192 50, T256  65
+//     1536 x  16384 -> 384           T128  35, T192Q 36, T192P 36, T192 30, T256  53
+//      192 x  65536 -> 768           T128  42, T192Q 35, T192P 31, T192 30, T256  52
+//     4096 x   8192 -> 4096          T128 287, T192Q 274, T192P 275, T192 278, T256 216
 static LinPlan plan_product(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
+    auto up = [](int64_t n, int b) { return (n + b - 1) / b; };
+    auto count = [&](Tile t) { return up(nq, kTiles[t].bq) * up(np, kTiles[t].bp); };
+    auto wide = [&](int64_t n) { return up(n, 192) * 192 <= up(n, 128) * 128; };     // 192 wastes no more than 128
     LinPlan pl;
-    pl.ke = 128 / elem_bytes;
-    auto count = [&](int b) { return ((nq + b - 1) / b) * ((np + b - 1) / b); };
-    const bool big = count(128) >= cus || (split && nq > 64 && np > 64);
-    pl.bp = pl.bq = big ? 128 : 64;
-    pl.tiles_p = (np + pl.bp - 1) / pl.bp;
-    pl.tiles = count(pl.bp);
-    pl.splits = 1;
-    const int64_t stages = (nk + pl.ke - 1) / pl.ke;
-    if (split) {
-        // two workgroups per CU, and at least 4 stages each
-        int64_t s = (2 * (int64_t)cus + pl.tiles - 1) / pl.tiles;
-        if (s > stages / 4) s = stages / 4;
-        if (s > 1) pl.splits = (int)s;
+    const int64_t big = count(T256), rounds = up(big, cus);
+    const bool small = nq <= 64 || np <= 64;
+    if (!small && big >= cus && big * 10 >= rounds * cus * 8 && nk * elem_bytes >= 1024 &&
+        (double)nq * np >= 0.8 * big * 256 * 256) {
+        pl.tile = T256;             // whole rounds of full tiles and a contraction that hides the ends
+    } else if (split) {
+        pl.tile = small ? T64 : wide(np) && np > 128 ? (wide(nq) && nq > 128 ? T192 : T192P) : (wide(nq) && nq > 128 ? T192Q : T128);
+    } else if (small || count(T128) < cus) {
+        pl.tile = T64;
+    } else if (nk * elem_bytes <= 384) {
+        pl.tile = T128S;
+    } else {
+        pl.tile = wide(np) && np > 128 ? T192P : T128;
     }
-    const int64_t per = (stages + pl.splits - 1) / pl.splits;
-    pl.k_per_split = per * pl.ke;
-    pl.splits = (int)((stages + per - 1) / per);
+    const TileShape& sh = kTiles[pl.tile];
+    const int ke = sh.kb / elem_bytes;
+    pl.tiles_p = (int)up(np, sh.bp);
+    pl.tiles = count(pl.tile);
+    const int64_t stages = up(nk, ke);
+    int64_t s = 1;
+    if (split && pl.tile != T256) {
+        // one round of workgroups (64-wide tiles: two), each with at least 4 stages
+        s = (pl.tile == T64 ? 2 : 1) * (int64_t)cus * (pl.tile == T192P || pl.tile == T192Q ? 2 : 1) / pl.tiles;
+        if (s > stages / 4) s = stages / 4;
+        if (s < 1) s = 1;
+    }
+    const int64_t per = up(stages, (int)s);
+    pl.k_per_split = per * ke;
+    pl.splits = (int)up(stages, (int)per);
     return pl;
 }
 
-template <int DT, bool PT, bool QT>
+static uint64_t reciprocal40(uint32_t d) { return ((1ull << 40) + d - 1) / d; }
+
+template <int DT, bool PT, bool QT, int ACT>
 static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t st) {
-    a.tiles = pl.tiles; a.tiles_p = pl.tiles_p; a.splits = pl.splits; a.k_per_split = pl.k_per_split;
+    a.tiles = (uint32_t)pl.tiles; a.tiles_p = pl.tiles_p; a.splits = pl.splits; a.k_per_split = pl.k_per_split;
+    a.by_tiles = reciprocal40(a.tiles); a.by_tiles_p = reciprocal40(a.tiles_p);
     const int64_t total = pl.tiles * pl.splits;
-    const dim3 grid((unsigned)(8 * ((total + 7) / 8))), block(256);
-    if (pl.bp == 128) {
-        if (vec) hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 128, 128, 2, 2, 128, 2, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 128, 128, 2, 2, 128, 2, false>), grid, block, 0, st, a);
-    } else {
-        if (vec) hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 64, 64, 2, 2, 128, 3, true>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 64, 64, 2, 2, 128, 2, false>), grid, block, 0, st, a);
+    const dim3 grid((unsigned)(8 * ((total + 7) / 8)));
+    constexpr bool TURNED = PT && QT;
+#define FWA2_GO(BP, BQ, WP, WQ, KB, ST, WAVES) \
+    hipLaunchKernelGGL((linear_kernel<DT, PT, QT, BP, BQ, WP, WQ, KB, ST, true, ACT, WAVES>), grid, dim3(64 * WP * WQ), 0, st, a)
+    if (!vec) {
+        // rows off 16-byte boundaries: through registers, on two tile sizes
+        if (kTiles[pl.tile].bp == 64) hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 64, 64, 2, 2, 64, 2, false, -1, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((linear_kernel<DT, PT, QT, 128, 128, 2, 2, 64, 2, false, -1, 1>), grid, dim3(256), 0, st, a);
+        return;
     }
+    switch (pl.tile) {
+        case T64: FWA2_GO(64, 64, 2, 2, 64, 4, 4); break;
+        case T128S:
+            if constexpr (!TURNED) FWA2_GO(128, 128, 2, 2, 64, 2, 3);
+            break;
+        case T128: FWA2_GO(128, 128, 2, 2, 128, 2, 2); break;
+        case T192P: FWA2_GO(192, 128, 2, 2, 128, 2, 2); break;
+        case T192Q:
+            if constexpr (TURNED) FWA2_GO(128, 192, 2, 2, 128, 2, 2);
+            break;
+        case T192:
+            if constexpr (TURNED) FWA2_GO(192, 192, 2, 2, 128, 2, 1);
+            break;
+        case T256: FWA2_GO(256, 256, 2, 4, 128, 2, 2); break;
+    }
+#undef FWA2_GO
+}
+
+// The activations a product is compiled for; the others are decided at run time, row by row of the epilogue.
+template <int DT>
+static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, hipStream_t st) {
+    if (a.act == FWA2_ACT_NONE) launch_product<DT, false, false, FWA2_ACT_NONE>(a, pl, vec, st);
+    else if (a.act == FWA2_ACT_GELU) launch_product<DT, false, false, FWA2_ACT_GELU>(a, pl, vec, st);
+    else launch_product<DT, false, false, -1>(a, pl, vec, st);
+}
+
+// Tiles for operands that go through registers.
+static LinPlan plan_unaligned(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
+    LinPlan pl = plan_product(nq, np, nk, split, elem_bytes, cus);
+    const int b = pl.tile == T64 ? 64 : 128;
+    pl.tile = b == 64 ? T64 : T128S;
+    pl.tiles_p = (np + b - 1) / b;
+    pl.tiles = (nq + b - 1) / b * pl.tiles_p;
+    const int64_t ke = 64 / elem_bytes, stages = (nk + ke - 1) / ke, per = (stages + pl.splits - 1) / pl.splits;
+    pl.k_per_split = per * ke;
+    pl.splits = (int)((stages + per - 1) / per);
+    return pl;
+}
+static LinPlan plan(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus, bool vec) {
+    return vec ? plan_product(nq, np, nk, split, elem_bytes, cus) : plan_unaligned(nq, np, nk, split, elem_bytes, cus);
 }
 
 static inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -649,14 +936,14 @@ static LinArgs forward_args(const fwa2_linear* p) {
     a.residual = reinterpret_cast<const char*>(p->residual); a.residual_stride = p->residual_stride * 2;
     a.q_scale = p->x_scale; a.p_scale = p->weight_scale;
     a.out_bf16 = p->dtype == FWA2_BF16;
-    a.out_vec = p->out_features % 8 == 0 && al16(p->y) && al16(p->z) && (!p->residual || rows16(p->residual, p->residual_stride, 8, 2));
+    a.out_vec = p->out_features % 8 == 0 && al16(p->y) && al16(p->z) && al16(p->bias) && (!p->residual || rows16(p->residual, p->residual_stride, 8, 2));
     return a;
 }
 
 #if FWA2_HALF == 3
 void linear_forward_e4m3(const fwa2_linear* p, int cus, hipStream_t st) {
     const bool vec = rows16(p->x, p->x_stride, p->in_features, 1) && rows16(p->weight, p->weight_stride, p->in_features, 1);
-    launch_product<FWA2_E4M3, false, false>(forward_args(p), plan_product(p->rows, p->out_features, p->in_features, false, 1, cus), vec, st);
+    launch_forward<FWA2_E4M3>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 1, cus, vec), vec, st);
 }
 #else
 #if FWA2_HALF == 1
@@ -668,7 +955,7 @@ void linear_forward_e4m3(const fwa2_linear* p, int cus, hipStream_t st) {
 #endif
 void FWA2_LIN_FN(linear_forward)(const fwa2_linear* p, int cus, hipStream_t st) {
     const bool vec = rows16(p->x, p->x_stride, p->in_features, 2) && rows16(p->weight, p->weight_stride, p->in_features, 2);
-    launch_product<FWA2_LIN_DT, false, false>(forward_args(p), plan_product(p->rows, p->out_features, p->in_features, false, 2, cus), vec, st);
+    launch_forward<FWA2_LIN_DT>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 2, cus, vec), vec, st);
 }
 void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st) {
     typedef Elem<FWA2_LIN_DT>::E E;
@@ -688,7 +975,7 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         dz_stride = n;
         ws += ((size_t)m * n * 2 + 255) / 256 * 256;
     }
-    const bool vec = rows16(dz, dz_stride, n, 2);
+    const bool dz_vec = rows16(dz, dz_stride, n, 2);
     if (p->dx != nullptr) {
         LinArgs a = {};
         a.q = dz; a.q_stride = dz_stride * 2;
@@ -696,8 +983,8 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         a.nq = m; a.np = k; a.nk = n;
         a.out = p->dx;
         a.out_vec = k % 8 == 0 && al16(p->dx);
-        launch_product<FWA2_LIN_DT, true, false>(a, plan_product(m, k, n, false, 2, cus),
-                                                 vec && rows16(p->weight, p->weight_stride, k, 2), st);
+        const bool vec = dz_vec && rows16(p->weight, p->weight_stride, k, 2);
+        launch_product<FWA2_LIN_DT, true, false, FWA2_ACT_NONE>(a, plan(m, k, n, false, 2, cus, vec), vec, st);
     }
     if (p->dweight != nullptr) {
         LinArgs a = {};
@@ -706,11 +993,12 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         a.nq = n; a.np = k; a.nk = m;
         a.out = p->dweight; a.db = p->dbias;
         a.out_vec = k % 8 == 0 && al16(p->dweight);
-        const LinPlan pl = plan_product(n, k, m, true, 2, cus);
+        const bool vec = dz_vec && rows16(p->x, p->x_stride, k, 2);
+        const LinPlan pl = plan(n, k, m, true, 2, cus, vec);
         const int64_t cells = (int64_t)n * k;
         a.part = reinterpret_cast<float*>(ws);
         a.part_db = a.part + (int64_t)pl.splits * cells;
-        launch_product<FWA2_LIN_DT, true, true>(a, pl, vec && rows16(p->x, p->x_stride, k, 2), st);
+        launch_product<FWA2_LIN_DT, true, true, FWA2_ACT_NONE>(a, pl, vec, st);
         if (pl.splits > 1) {
             const int64_t blocks = (cells + 255) / 256 + (p->dbias ? (n + 255) / 256 : 0);
             hipLaunchKernelGGL(linear_sum_kernel<E>, dim3((unsigned)blocks), dim3(1024), 0, st, a.part, a.part_db, pl.splits,
@@ -729,8 +1017,13 @@ size_t linear_workspace_bytes(const fwa2_linear* p, bool backward, int cus) {
     if (!backward) return 0;
     size_t need = p->activation != FWA2_ACT_NONE ? ((size_t)p->rows * p->out_features * 2 + 255) / 256 * 256 : 0;
     if (p->dweight != nullptr) {
-        const LinPlan pl = plan_product(p->out_features, p->in_features, p->rows, true, 2, cus);
-        if (pl.splits > 1) need += (size_t)pl.splits * p->out_features * ((size_t)p->in_features + 1) * sizeof(float);
+        // whichever way the operands turn out to be read
+        int splits = 1;
+        for (bool vec : {false, true}) {
+            const LinPlan pl = plan(p->out_features, p->in_features, p->rows, true, 2, cus, vec);
+            if (pl.splits > splits) splits = pl.splits;
+        }
+        if (splits > 1) need += (size_t)splits * p->out_features * ((size_t)p->in_features + 1) * sizeof(float);
     }
     return need;
 }

@@ -297,8 +297,7 @@ int fwa2_cpb_bias_backward(const void* table, const void* dbias, int dtype, int 
  * The rest of a transformer block: normalisation with the residual's addition, matrix products with an epilogue, and
  * the 8-bit forms of both.  The reference composes these from framework calls (nn.LayerNorm, nn.Linear, nn.GELU and
  * the additions of flash_win_attn_v2/swin_transformer_v2.py:66-85, 443-445).  The conventions at the top of this file
- * hold; rows are the flattened leading dimensions of a tensor, their innermost stride is 1, and
- * both extents of a matrix are at most 2^24 - 1 (weights) respectively 2^31 - 1 (rows).
+ * hold; rows are the flattened leading dimensions of a tensor and their innermost stride is 1.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* 8-bit floats with 4 exponent and 3 mantissa bits, no infinities, largest value 448 (the OCP encoding). */
@@ -402,8 +401,8 @@ typedef struct fwa2_linear {
     int32_t dtype;          /* FWA2_F16 or FWA2_BF16: bias, residual, y, z and all gradients */
     int32_t x_dtype;        /* of x and weight: `dtype` or FWA2_E4M3 */
     int32_t activation;     /* fwa2_activation */
-    int32_t in_features;    /* 1 .. 2^24 - 1 */
-    int32_t out_features;   /* 1 .. 2^24 - 1 */
+    int32_t in_features;    /* 1 .. 2^22 - 1 */
+    int32_t out_features;   /* 1 .. 2^22 - 1 */
     int32_t reserved;       /* 0 */
     int64_t rows;           /* 1 .. 2^31 - 1 */
 

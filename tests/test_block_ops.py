@@ -156,7 +156,8 @@ def test_linear_validate(lib):
         refuse("positive", **{field: 0})
         refuse("positive", **{field: -3})
     refuse("positive", rows=1 << 31)
-    refuse("too large", no, in_features=1 << 24, x_stride=1 << 24, weight_stride=1 << 24)
+    refuse("too large", no, in_features=1 << 22, x_stride=1 << 22, weight_stride=1 << 22)
+    refuse("too large", no, out_features=1 << 22, residual_stride=1 << 22)
     refuse("too large", no, rows=(1 << 31) - 1, out_features=1 << 20)
     refuse("x: null", x=0)
     refuse("weight: null", weight=0)
