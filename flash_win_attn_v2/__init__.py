@@ -5,8 +5,8 @@ import sys
 
 import flash_window_attention_v2_amd as _impl
 from flash_window_attention_v2_amd import (FlashWindowAttentionV2, FlashWindowAttentionV2Grid,
-                                           FlashWindowAttentionV2QKVPacked, FusedLinear, ResidualNorm, SwinTransformerV2,
-                                           WindowAttention, flash_win_attn_v2_func, flash_win_attn_v2_grid_func,
+                                           FlashWindowAttentionV2QKVPacked, SwinTransformerV2, WindowAttention,
+                                           flash_win_attn_v2_func, flash_win_attn_v2_grid_func,
                                            flash_win_attn_v2_qkvpacked_func, fused_linear_fp8_func, fused_linear_func,
                                            quantize_rows_func, residual_norm_fp8_func, residual_norm_func,
                                            win_attention_torch, win_attention_torch_compile)

@@ -7,13 +7,13 @@ from .win_attention_func import (flash_win_attn_v2_func, flash_win_attn_v2_grid_
                                  win_attention_torch, win_attention_torch_compile)
 from .flash_window_attention_v2 import (FlashWindowAttentionV2, FlashWindowAttentionV2Grid,
                                          FlashWindowAttentionV2QKVPacked)
-from .block_ops import (FusedLinear, ResidualNorm, fused_linear_fp8_func, fused_linear_func, quantize_rows_func,
-                        residual_norm_fp8_func, residual_norm_func)
+from .block_ops import (fused_linear_fp8_func, fused_linear_func, quantize_rows_func, residual_norm_fp8_func,
+                        residual_norm_func)
 from .swin_transformer_v2 import WindowAttention, SwinTransformerV2
 
 __all__ = ["flash_win_attn_v2_func", "flash_win_attn_v2_qkvpacked_func", "flash_win_attn_v2_grid_func",
            "win_attention_torch", "win_attention_torch_compile", "FlashWindowAttentionV2",
            "FlashWindowAttentionV2QKVPacked", "FlashWindowAttentionV2Grid",
-           "FusedLinear", "ResidualNorm", "fused_linear_func", "fused_linear_fp8_func", "quantize_rows_func",
+           "fused_linear_func", "fused_linear_fp8_func", "quantize_rows_func",
            "residual_norm_func", "residual_norm_fp8_func",
            "WindowAttention", "SwinTransformerV2"]

@@ -6,6 +6,7 @@ reported instead of being mis-read.  There is no fallback: if the shared
 library is missing every operator call raises.
 """
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -183,6 +184,32 @@ def load():
             raise Fwa2Error(f"libfwa2 ABI {lib.fwa2_abi_version()} != binding ABI {ABI_VERSION}")
         _lib = lib
     return _lib
+
+
+_EXT_PATH = os.path.join(os.path.dirname(_LIB_PATH), "_fwa2_torch.so")
+_ext = None
+
+
+def load_ext():
+    """The torch binding of the operators around the attention call (csrc/fwa2_torch.cpp), loaded once; raises if it has
+    not been built.  It links to the same libfwa2.so."""
+    global _ext
+    if _ext is not None:
+        return _ext
+    load()
+    with _lock:
+        if _ext is None:
+            if not os.path.exists(_EXT_PATH):
+                raise Fwa2Error(f"{_EXT_PATH} is missing: build it with `make -C {os.path.dirname(_LIB_PATH)}/../csrc` "
+                                "(or `python -c 'import __graft_entry__ as g; g.build()'`). There is no fallback path.")
+            import torch  # noqa: F401  (its libraries, before the module that links to them)
+            spec = importlib.util.spec_from_file_location("_fwa2_torch", _EXT_PATH)
+            ext = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ext)
+            if ext.abi_version() != ABI_VERSION:
+                raise Fwa2Error(f"_fwa2_torch ABI {ext.abi_version()} != binding ABI {ABI_VERSION}")
+            _ext = ext
+    return _ext
 
 
 def new_problem():

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import flash_window_attention_v2_amd as fwa2
-from flash_window_attention_v2_amd import _abi, block_ops
+from flash_window_attention_v2_amd import _abi
 
 FAKE = 0x100000     # never dereferenced by a validation
 
@@ -220,17 +220,18 @@ def test_python_refusals_without_a_gpu():
         fwa2.quantize_rows_func(torch.zeros(4, 0))
 
 
-def test_rows_are_views_where_they_can_be():
+def test_rows_are_views_where_they_can_be(lib):
+    as_rows = _abi.load_ext().rows
     a = torch.zeros(4, 6, 40)
     for t, stride, view in [(a, 40, True), (a[..., 3:20], 40, True), (a[:, :, ::2], 20, False), (a[0], 40, True),
                             (a[:, 0], 240, True), (a[:, :3], 40, False), (a[:1, :1], 40, True), (a[0, 0], 40, True),
                             (a[:, :1].expand(4, 6, 40), 40, False), (a.transpose(1, 2), 6, False)]:
-        rows, got = block_ops._rows(t)
+        rows, got = as_rows(t)
         assert rows.dim() == 2 and rows.shape == (t.numel() // t.shape[-1], t.shape[-1]) and got == stride
         assert (rows.untyped_storage().data_ptr() == a.untyped_storage().data_ptr()) == view
         assert torch.equal(rows.reshape(t.shape), t)
     far = torch.zeros(8).as_strided((1, 8), (1 << 30, 1))
-    assert block_ops._rows(far)[1] == 8         # the stride of a single row means nothing
+    assert as_rows(far)[1] == 8         # the stride of a single row means nothing
 
 
 def test_struct_sizes_match_the_header(lib):
