@@ -466,7 +466,12 @@ static int validate_norm(const fwa2_norm* p, int backward) {
         return FWA2_OK;
     }
     if (pre) {
-        if ((rc = check_ptr("h", p->h, sb))) return rc;
+        if (p->stream_dtype == FWA2_F32) {
+            if ((rc = check_ptr("h", p->h, sb))) return rc;
+        } else if ((rc = check_rows("x", p->x, p->x_stride, p->dim, xb)) ||
+                   (rc = check_rows("shortcut", p->shortcut, p->shortcut_stride, p->dim, sb))) {
+            return rc;
+        }
         if (p->dy && (rc = check_rows("dy", p->dy, p->dy_stride, p->dim, yb))) return rc;
         if (p->dh && (rc = check_rows("dh", p->dh, p->dh_stride, p->dim, sb))) return rc;
         if (p->dshortcut && (rc = check_ptr("dshortcut", p->dshortcut, sb))) return rc;

@@ -722,30 +722,31 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
 }
 
 #if FWA2_HALF != 3
-// dW, db = sums of the partial tiles, rounded once.  A workgroup owns 256 values; its 16 wavefronts take every 16th partial
-// (a fixed assignment) and their sums are added in order.
+// dW, db = sums of partial rows, rounded once.  A workgroup owns 256 values; its 16 wavefronts take every 16th partial (a
+// fixed assignment) and their sums are added in order.
 template <class E>
-__global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, const float* part_db, int splits, int64_t cells,
-                                                          int64_t nq, E* out, E* db) {
+__global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, int parts, const float* part_db, int parts_db,
+                                                          int64_t cells, int64_t nq, E* out, E* db) {
     __shared__ float s[16][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t blocks = (cells + 255) / 256;
     const bool rows = blockIdx.x >= blocks;         // the workgroups behind those of dW sum db
     const float* src = rows ? part_db : part;
+    const int n_parts = rows ? parts_db : parts;
     const int64_t n = rows ? nq : cells;
     const int64_t i0 = (rows ? blockIdx.x - blocks : (int64_t)blockIdx.x) * 256 + 4 * lane;
     float t[4] = {0.f, 0.f, 0.f, 0.f};
     if (n % 4 == 0) {
         if (i0 < n) {
-#pragma unroll 4
-            for (int k = wave; k < splits; k += 16) {
+#pragma unroll 8
+            for (int k = wave; k < n_parts; k += 16) {
                 const f32x4 v = *reinterpret_cast<const f32x4*>(src + (int64_t)k * n + i0);
 #pragma unroll
                 for (int j = 0; j < 4; j++) t[j] += v[j];
             }
         }
     } else {
-        for (int k = wave; k < splits; k += 16)
+        for (int k = wave; k < n_parts; k += 16)
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (i0 + j < n) t[j] += src[(int64_t)k * n + i0 + j];
@@ -763,29 +764,77 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, con
     }
 }
 
-// dz = dy act'(z), contiguous.
-template <class E>
+// dz = dy act'(z), contiguous, and the column sums of dz before its rounding (part_db, one partial row per blockIdx.y).
+// A workgroup owns up to 512 columns (8 per lane, `lanes` lanes a row, a power of two) and a stretch of rows; bound by its
+// three streams.
+constexpr int kActRows = 1024;      // at most so many stretches of rows: their partial sums stay small
+template <class E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t dy_stride, const E* z, E* dz, int64_t rows,
-                                                           int n, int act, int vec) {
+                                                           int n, int lanes, int64_t rows_per_block, float* part_db, int act) {
     typedef E V8 __attribute__((ext_vector_type(8)));
-    const int chunks = (n + 7) / 8;
-    const int64_t total = rows * chunks;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / chunks;
-        const int c = (int)(i - row * chunks) * 8;
-        const E* a = dy + row * dy_stride + c;
-        const E* b = z + row * n + c;
-        E* o = dz + row * n + c;
-        if (vec) {
-            const V8 g = *reinterpret_cast<const V8*>(a), v = *reinterpret_cast<const V8*>(b);
-            V8 r;
+    __shared__ float sums[256][9];
+    const int cl = threadIdx.x % lanes, rl = threadIdx.x / lanes, step = 256 / lanes;
+    const int c = (blockIdx.x * lanes + cl) * 8;
+    const int64_t r0 = blockIdx.y * rows_per_block, r1 = r0 + rows_per_block < rows ? r0 + rows_per_block : rows;
+    float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) r[j] = (E)((float)g[j] * slope_of((float)v[j], act));
-            *reinterpret_cast<V8*>(o) = r;
-        } else {
-            for (int j = 0; j < 8 && c + j < n; j++) o[j] = (E)((float)a[j] * slope_of((float)b[j], act));
+    for (int j = 0; j < 8; j++) t[j] = 0.f;
+    if (c < n) {
+#pragma unroll 4
+        for (int64_t row = r0 + rl; row < r1; row += step) {
+            const E* a = dy + row * dy_stride + c;
+            const E* b = z + row * n + c;
+            E* o = dz + row * n + c;
+            if (VEC) {
+                const V8 g = *reinterpret_cast<const V8*>(a), v = *reinterpret_cast<const V8*>(b);
+                V8 r;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float d = (float)g[j] * slope_of((float)v[j], ACT >= 0 ? ACT : act);
+                    t[j] += d;
+                    r[j] = (E)d;
+                }
+                *reinterpret_cast<V8*>(o) = r;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (c + j >= n) continue;
+                    const float d = (float)a[j] * slope_of((float)b[j], ACT >= 0 ? ACT : act);
+                    t[j] += d;
+                    o[j] = (E)d;
+                }
+            }
         }
     }
+    if (part_db == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < 8; j++) sums[threadIdx.x][j] = t[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < lanes * 8; i += 256) {
+        const int col = blockIdx.x * lanes * 8 + i;
+        if (col >= n) continue;
+        float v = 0.f;
+        for (int k = 0; k < step; k++) v += sums[k * lanes + (i >> 3)][i & 7];
+        part_db[(int64_t)blockIdx.y * n + col] = v;
+    }
+}
+struct ActPlan {
+    int lanes, blocks_x, blocks_y;
+    int64_t rows_per_block;
+};
+static ActPlan plan_act(int64_t rows, int n, int cus) {
+    ActPlan pl;
+    const int chunks = (n + 7) / 8;
+    pl.lanes = 1;
+    while (pl.lanes < 64 && pl.lanes < chunks) pl.lanes *= 2;
+    pl.blocks_x = (chunks + pl.lanes - 1) / pl.lanes;
+    int64_t y = (8 * (int64_t)cus + pl.blocks_x - 1) / pl.blocks_x;
+    if (y > kActRows) y = kActRows;
+    const int64_t step = 256 / pl.lanes, most = (rows + step - 1) / step;
+    if (y > most) y = most;
+    pl.rows_per_block = (rows + y - 1) / y;
+    pl.blocks_y = (int)((rows + pl.rows_per_block - 1) / pl.rows_per_block);
+    return pl;
 }
 #endif
 
@@ -957,6 +1006,11 @@ void FWA2_LIN_FN(linear_forward)(const fwa2_linear* p, int cus, hipStream_t st) 
     const bool vec = rows16(p->x, p->x_stride, p->in_features, 2) && rows16(p->weight, p->weight_stride, p->in_features, 2);
     launch_forward<FWA2_LIN_DT>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 2, cus, vec), vec, st);
 }
+static size_t dz_bytes(int64_t m, int n) { return ((size_t)m * n * 2 + 255) / 256 * 256; }
+static size_t act_bytes(const fwa2_linear* p, int cus) {
+    if (p->activation == FWA2_ACT_NONE || p->dbias == nullptr) return 0;
+    return ((size_t)plan_act(p->rows, p->out_features, cus).blocks_y * p->out_features * sizeof(float) + 255) / 256 * 256;
+}
 void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st) {
     typedef Elem<FWA2_LIN_DT>::E E;
     const int64_t m = p->rows;
@@ -964,16 +1018,25 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
     const char* dz = reinterpret_cast<const char*>(p->dy);
     int64_t dz_stride = p->dy_stride;
     char* ws = reinterpret_cast<char*>(p->workspace);
+    float* part_act = nullptr;      // of dbias, from the unrounded dz
+    ActPlan act = {};
     if (p->activation != FWA2_ACT_NONE) {
-        const int64_t chunks = m * ((n + 7) / 8);
-        const int64_t blocks = (chunks + 255) / 256, most = 16 * (int64_t)cus;
-        const int vec = rows16(p->dy, p->dy_stride, n, 2) && al16(p->z);
-        hipLaunchKernelGGL(act_backward_kernel<E>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st,
-                           reinterpret_cast<const E*>(p->dy), p->dy_stride, reinterpret_cast<const E*>(p->z),
-                           reinterpret_cast<E*>(ws), m, n, p->activation, vec);
+        act = plan_act(m, n, cus);
+        if (p->dbias != nullptr) part_act = reinterpret_cast<float*>(ws + dz_bytes(m, n));
+        const dim3 grid(act.blocks_x, act.blocks_y), block(256);
+        const bool vec = rows16(p->dy, p->dy_stride, n, 2) && al16(p->z);
+        const E *dy = reinterpret_cast<const E*>(p->dy), *z = reinterpret_cast<const E*>(p->z);
+#define FWA2_GO(ACT, VEC) hipLaunchKernelGGL((act_backward_kernel<E, ACT, VEC>), grid, block, 0, st, dy, p->dy_stride, z, \
+                                             reinterpret_cast<E*>(ws), m, n, act.lanes, act.rows_per_block, part_act, p->activation)
+        if (!vec) FWA2_GO(-1, false);
+        else if (p->activation == FWA2_ACT_GELU) FWA2_GO(FWA2_ACT_GELU, true);
+        else if (p->activation == FWA2_ACT_GELU_TANH) FWA2_GO(FWA2_ACT_GELU_TANH, true);
+        else if (p->activation == FWA2_ACT_SILU) FWA2_GO(FWA2_ACT_SILU, true);
+        else FWA2_GO(FWA2_ACT_RELU, true);
+#undef FWA2_GO
         dz = ws;
         dz_stride = n;
-        ws += ((size_t)m * n * 2 + 255) / 256 * 256;
+        ws += dz_bytes(m, n) + act_bytes(p, cus);
     }
     const bool dz_vec = rows16(dz, dz_stride, n, 2);
     if (p->dx != nullptr) {
@@ -991,7 +1054,8 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         a.q = dz; a.q_stride = dz_stride * 2;
         a.p = reinterpret_cast<const char*>(p->x); a.p_stride = p->x_stride * 2;
         a.nq = n; a.np = k; a.nk = m;
-        a.out = p->dweight; a.db = p->dbias;
+        a.out = p->dweight;
+        a.db = part_act ? nullptr : p->dbias;
         a.out_vec = k % 8 == 0 && al16(p->dweight);
         const bool vec = dz_vec && rows16(p->x, p->x_stride, k, 2);
         const LinPlan pl = plan(n, k, m, true, 2, cus, vec);
@@ -999,10 +1063,13 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         a.part = reinterpret_cast<float*>(ws);
         a.part_db = a.part + (int64_t)pl.splits * cells;
         launch_product<FWA2_LIN_DT, true, true, FWA2_ACT_NONE>(a, pl, vec, st);
-        if (pl.splits > 1) {
-            const int64_t blocks = (cells + 255) / 256 + (p->dbias ? (n + 255) / 256 : 0);
-            hipLaunchKernelGGL(linear_sum_kernel<E>, dim3((unsigned)blocks), dim3(1024), 0, st, a.part, a.part_db, pl.splits,
-                               cells, (int64_t)n, reinterpret_cast<E*>(p->dweight), reinterpret_cast<E*>(p->dbias));
+        const int64_t summed = pl.splits > 1 ? cells : 0;
+        const bool sum_db = p->dbias != nullptr && (part_act || pl.splits > 1);
+        if (summed || sum_db) {
+            const int64_t blocks = (summed + 255) / 256 + (sum_db ? (n + 255) / 256 : 0);
+            hipLaunchKernelGGL(linear_sum_kernel<E>, dim3((unsigned)blocks), dim3(1024), 0, st, a.part, pl.splits,
+                               part_act ? part_act : a.part_db, part_act ? act.blocks_y : pl.splits, summed, (int64_t)n,
+                               reinterpret_cast<E*>(p->dweight), reinterpret_cast<E*>(p->dbias));
         }
     }
 }
@@ -1015,7 +1082,7 @@ void linear_forward_e4m3(const fwa2_linear* p, int cus, hipStream_t st);
 
 size_t linear_workspace_bytes(const fwa2_linear* p, bool backward, int cus) {
     if (!backward) return 0;
-    size_t need = p->activation != FWA2_ACT_NONE ? ((size_t)p->rows * p->out_features * 2 + 255) / 256 * 256 : 0;
+    size_t need = p->activation != FWA2_ACT_NONE ? dz_bytes(p->rows, p->out_features) + act_bytes(p, cus) : 0;
     if (p->dweight != nullptr) {
         // whichever way the operands turn out to be read
         int splits = 1;

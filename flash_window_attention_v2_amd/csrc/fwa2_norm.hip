@@ -19,6 +19,8 @@
 // A workgroup walks over rows with a stride of the grid and asks for its next row before it works on the present one.
 // Its lanes keep their columns, so weight and bias are read once and the column sums dw, db stay in registers until the
 // end; one partial row per workgroup then goes to the workspace and a second kernel adds those in a fixed order.
+#include <type_traits>
+
 #include "fwa2_common.hpp"
 
 namespace fwa2 {
@@ -310,11 +312,13 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_fwd_kernel(const NormArg
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------
-// The rows' source v: x (POST) or the saved h (PRE).  In the PRE form h was rounded to the stream's type when it was
-// saved, its statistics were not: v^ is off by half a step of that type, as in any norm whose input is kept in it.
+// The rows' source v: x (POST); the saved h where the stream is fp32 (PRE); s + g x once more where it is not: h was rounded
+// to 16 bits when it left the forward call, and v^ taken from it would carry that rounding into every sum over the rows
+// (dweight 1.4 times as far from the exact one as its own rounding puts it) for one read less of nine.
 template <class XT, class ST, bool PRE, int LPR, int CPL, bool VEC>
 __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArgs a) {
-    typedef typename std::conditional<PRE, ST, XT>::type VT;       // of v
+    constexpr bool TWO = PRE && !std::is_same<ST, float>::value;    // v = s + g x
+    typedef typename std::conditional<PRE, ST, XT>::type VT;       // of v (of s)
     typedef typename std::conditional<PRE, XT, ST>::type YT;       // of dy
     constexpr int RPB = norm_block(LPR) / LPR;
     __shared__ uint32_t red[32];
@@ -334,15 +338,23 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArg
     }
 
     typename Vec8<VT>::V vr[CPL];
+    typename Vec8<XT>::V xr[TWO ? CPL : 1];
     typename Vec8<YT>::V yr[CPL];
     typename Vec8<ST>::V hr[PRE ? CPL : 1];
     float2 st;
     auto fetch = [&](int64_t row) __attribute__((always_inline)) {
-        const VT* vp = PRE ? reinterpret_cast<const VT*>(a.h) + row * dim : reinterpret_cast<const VT*>(a.x) + row * a.xs;
+        const VT* vp = TWO   ? reinterpret_cast<const VT*>(a.s) + row * a.ss
+                       : PRE ? reinterpret_cast<const VT*>(a.h) + row * dim
+                             : reinterpret_cast<const VT*>(a.x) + row * a.xs;
         const YT* yp = reinterpret_cast<const YT*>(a.dy) + row * a.dys;
         st = a.stats[row];
 #pragma unroll
         for (int c = 0; c < CPL; c++) vr[c] = row_load8<VEC>(vp, 8 * (c * LPR + l), dim);
+        if (TWO) {
+            const XT* xp = reinterpret_cast<const XT*>(a.x) + row * a.xs;
+#pragma unroll
+            for (int c = 0; c < CPL; c++) xr[TWO ? c : 0] = row_load8<VEC>(xp, 8 * (c * LPR + l), dim);
+        }
         if (!PRE || a.dy != nullptr) {
 #pragma unroll
             for (int c = 0; c < CPL; c++) yr[c] = row_load8<VEC>(yp, 8 * (c * LPR + l), dim);
@@ -375,7 +387,9 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArg
         for (int c = 0; c < CPL; c++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float vh = ((float)vr[c][j] - m) * r;
+                float src = (float)vr[c][j];
+                if (TWO) src += g * (float)xr[TWO ? c : 0][j];
+                const float vh = (src - m) * r;
                 // a copy of the last row adds nothing to the column sums
                 const float dn = ok ? (PRE ? (float)yr[c][j] : g * (float)yr[c][j]) : 0.f;
                 dw[c][j] += dn * vh;
@@ -655,7 +669,9 @@ hipError_t launch_norm_forward(const fwa2_norm* p, int cus, hipStream_t st) {
 hipError_t launch_norm_backward(const fwa2_norm* p, int cus, hipStream_t st) {
     const NormArgs a = norm_args(p);
     const bool pre = p->placement == FWA2_NORM_PRE;
-    const bool vec = p->dim % 8 == 0 && (pre ? al16(p->h) : al16(p->x) && p->x_stride % 8 == 0) &&
+    const bool two = pre && p->stream_dtype != FWA2_F32;
+    const bool vec = p->dim % 8 == 0 && (!pre || two ? al16(p->x) && p->x_stride % 8 == 0 : al16(p->h)) &&
+                     (!two || (al16(p->shortcut) && p->shortcut_stride % 8 == 0)) &&
                      (!p->dy || (al16(p->dy) && p->dy_stride % 8 == 0)) && (!pre || !p->dh || (al16(p->dh) && p->dh_stride % 8 == 0)) &&
                      al16(p->dx) && (!pre || al16(p->dshortcut));
     const bool s32 = p->stream_dtype == FWA2_F32;

@@ -206,6 +206,8 @@ struct NormHow {
     int kind, place;
     at::ScalarType x, stream;
     bool pre() const { return place == FWA2_NORM_PRE; }
+    bool exact_h() const { return pre() && stream == at::kFloat; }
+    bool two() const { return pre() && stream != at::kFloat; }
 };
 struct NormParams {     // weight, bias and gate, contiguous, for as long as the call needs them
     Tensor weight, bias, gate;
@@ -265,8 +267,9 @@ struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Optional& shortcut, const Optional& bias,
                                  const Optional& gate, const NormHow& how) {
         const NormOut o = norm_forward(x, shortcut, weight, bias, gate, how, true, false);
-        // kept for the backward pass: x (post) or the h returned (pre), and two numbers per row
-        ctx->save_for_backward({how.pre() ? o.h : x, weight, value(bias), value(gate), o.stats});
+        // kept for the backward pass: x (post), the h returned (pre over an fp32 stream) or x and shortcut (pre over a 16-bit
+        // one, whose h was rounded), and two numbers per row
+        ctx->save_for_backward({how.exact_h() ? o.h : x, weight, value(bias), value(gate), o.stats, how.two() ? value(shortcut) : Tensor()});
         ctx->saved_data["eps"] = how.eps;
         ctx->saved_data["how"] = (int64_t)(how.kind + 2 * how.place + 4 * (shortcut ? 1 : 0) + 8 * (bias ? 1 : 0) + 16 * (int)how.x + 4096 * (int)how.stream);
         ctx->set_materialize_grads(false);
@@ -275,7 +278,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &v = saved[0], &weight = saved[1], &bias = saved[2], &gate = saved[3], &stats = saved[4];
+        const Tensor &v = saved[0], &weight = saved[1], &bias = saved[2], &gate = saved[3], &stats = saved[4], &shortcut = saved[5];
         const int64_t code = ctx->saved_data["how"].toInt();
         const NormHow how = {ctx->saved_data["eps"].toDouble(), (int)(code & 1), (int)(code >> 1 & 1), (at::ScalarType)(code / 16 % 256),
                              (at::ScalarType)(code / 4096)};
@@ -300,14 +303,15 @@ struct NormNode : torch::autograd::Function<NormNode> {
             } else if (dx.defined() || ds.defined() || dw.defined() || db.defined()) {
                 NormParams keep;
                 fwa2_norm p = norm_description(v, how, weight, bias, gate, keep);
-                Rows vr, dyr, dhr;
-                if (how.pre()) {
+                Rows vr, sr, dyr, dhr;
+                if (how.exact_h()) {
                     p.h = ptr(v);       // an output of the forward call: contiguous
-                    if (dh.defined()) { dhr = Rows(dh); p.dh = dhr.ptr; p.dh_stride = dhr.stride; }
                 } else {
                     vr = Rows(v);
                     p.x = vr.ptr; p.x_stride = vr.stride;
                 }
+                if (how.two()) { sr = Rows(shortcut); p.shortcut = sr.ptr; p.shortcut_stride = sr.stride; }
+                if (dh.defined()) { dhr = Rows(dh); p.dh = dhr.ptr; p.dh_stride = dhr.stride; }
                 if (dy.defined()) { dyr = Rows(dy); p.dy = dyr.ptr; p.dy_stride = dyr.stride; }
                 p.stats = (float*)ptr(stats);
                 p.dx = ptr(dx); p.dshortcut = ptr(ds); p.dweight = ptr(dw); p.dbias = ptr(db);

@@ -337,9 +337,9 @@ typedef struct fwa2_norm {
     int32_t dim;            /* 1 .. FWA2_NORM_MAX_DIM */
     int32_t gate_dtype;     /* `dtype` or FWA2_F32 */
 
-    const void* x;          /* [rows, dim], rows x_stride elements apart; backward (PRE): not read */
+    const void* x;          /* [rows, dim], rows x_stride elements apart */
     int64_t     x_stride;
-    const void* shortcut;   /* [rows, dim]; NULL only in the POST form; backward: not read */
+    const void* shortcut;   /* [rows, dim]; NULL only in the POST form */
     int64_t     shortcut_stride;
     const void* weight;     /* [dim] */
     const void* bias;       /* [dim] or NULL */
@@ -347,13 +347,14 @@ typedef struct fwa2_norm {
     int64_t     rows_per_gate;
 
     void*  y;               /* [rows, dim] contiguous; NULL with the 8-bit output of the PRE form */
-    void*  h;               /* PRE: [rows, dim] contiguous.  Backward: the h that the forward call wrote */
+    void*  h;               /* PRE: [rows, dim] contiguous */
     void*  y8;              /* optional [rows, dim] contiguous e4m3: y divided by its row's scale; forward only */
     float* y8_scale;        /* [rows], with y8: max(max |y| of the row, 2^-100) * fp32(1 / 448) */
     float* stats;           /* [rows, 2] mean (0 for RMS) and 1 / sqrt(..) of each row: forward writes them unless
                                NULL, backward reads them */
 
-    /* (backward) */
+    /* (backward; it reads x in the POST form, the h of the forward call in the PRE form with stream_dtype FWA2_F32,
+       and x and shortcut in the PRE form otherwise) */
     const void* dy;         /* [rows, dim] gradient of y, or NULL = zero (PRE only) */
     int64_t     dy_stride;
     const void* dh;         /* PRE: gradient of h, or NULL = zero */

@@ -79,9 +79,8 @@ def norm_ref(x, shortcut, weight, bias, eps, kind, placement, gate, dy=None, dh=
     DY = dy.double() if dy is not None else torch.zeros_like(X)
     dn = DY if pre else g * DY
     t = dn * W
-    if pre:         # backward starts from the saved h, rounded to the stream's type
-        saved = v.abs() * half_step(s_t) + tiny(s_t)
-        vh_off = vh_off + saved * r
+    if pre and s_t == torch.float32:        # backward starts from the saved h, rounded to the stream's type
+        vh_off = vh_off + (v.abs() * half_step(s_t) + tiny(s_t)) * r
     t_off = 2 * U * t.abs()
     c1 = t.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(mean)
     c1_off = n_sum * t.abs().mean(-1, keepdim=True) if kind == "layer" else 0.0

@@ -86,7 +86,9 @@ def test_norm_validate(lib):
     refuse("workspace", backward=1, workspace=0)
     refuse("need", backward=1, workspace_bytes=8)
     refuse("aligned", backward=1, workspace=FAKE + 8)
-    refuse("h: null", backward=1, pre=True, h=0)
+    refuse("h: null", backward=1, pre=True, h=0, stream_dtype=_abi.F32)
+    refuse("x: null", backward=1, pre=True, x=0)
+    refuse("shortcut: null", backward=1, pre=True, shortcut=0)
     p = _norm(True, True)       # both incoming gradients may be absent on their own
     p.dy = 0
     assert check(p, 1) == _abi.OK
