@@ -721,13 +721,112 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
     }
 }
 
+// ---- few rows ---------------------------------------------------------------------------------------------------
+// Up to 64 rows (single tokens, a pooled image): the call reads the weights once and is over; what counts is how soon every
+// load is on its way.  A workgroup owns 16 output columns and its wavefronts split the contraction; operands go from memory
+// straight into the registers of 16-row products (no staging, no barrier until the end), partial sums meet in LDS and are
+// added in a fixed order.  1 x 768 -> 1000: 9.0 us on 64 x 64 tiles (24 stages one after the other), see the table at
+// plan_product for the rest.
+template <int DT> struct Frag16 {           // v_mfma_f32_16x16x32
+    typedef typename Elem<DT>::V8 V;
+    static constexpr int BYTES = 64;        // of a row per product
+    static __device__ __forceinline__ V load(const char* row, int64_t left, int g) {
+        if (16 * g < left) return *reinterpret_cast<const V*>(row + 16 * g);
+        return zero8<V>();
+    }
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) { return Elem<DT>::mfma16(a, b, c); }
+};
+template <> struct Frag16<FWA2_E4M3> {      // v_mfma_f32_16x16x128
+    typedef i32x8 V;
+    static constexpr int BYTES = 128;
+    static __device__ __forceinline__ V load(const char* row, int64_t left, int g) {
+        u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+        if (16 * g < left) a = *reinterpret_cast<const u32x4*>(row + 16 * g);
+        if (64 + 16 * g < left) b = *reinterpret_cast<const u32x4*>(row + 64 + 16 * g);
+        V v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[i] = (int)a[i]; v[4 + i] = (int)b[i]; }
+        return v;
+    }
+    static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+    }
+};
+constexpr int kRowsMax = 64, kRowsWaves = 16;
+
+template <int DT, int MQ>       // MQ: groups of 16 rows
+__global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinArgs a) {
+    typedef Frag16<DT> F;
+    constexpr int EB = LinElem<DT>::bytes, U = MQ == 1 ? 8 : 4;
+    __shared__ float sums[kRowsWaves][MQ][16][17];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int l16 = lane & 15, g = lane >> 4;
+    const int p0 = blockIdx.x * 16;
+    const char* prow = a.p + (int64_t)min(p0 + l16, a.np - 1) * a.p_stride;
+    const char* qrow[MQ];
+#pragma unroll
+    for (int i = 0; i < MQ; i++) qrow[i] = a.q + (int64_t)min(16 * i + l16, (int)a.nq - 1) * a.q_stride;
+    f32x4 acc[MQ];
+#pragma unroll
+    for (int i = 0; i < MQ; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t bytes = a.nk * EB;
+    const int64_t steps = (bytes + F::BYTES - 1) / F::BYTES;
+    // every `waves`-th product is this wavefront's: neighbouring wavefronts read neighbouring stretches
+    for (int64_t s = wave; s < steps; s += (int64_t)waves * U) {
+        typename F::V fp[U], fq[U][MQ];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t at = (s + (int64_t)u * waves) * F::BYTES;     // beyond the end: zeros
+            fp[u] = F::load(prow + at, bytes - at, g);
+#pragma unroll
+            for (int i = 0; i < MQ; i++) fq[u][i] = F::load(qrow[i] + at, bytes - at, g);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < MQ; i++) acc[i] = F::mfma(fp[u], fq[u][i], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < MQ; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sums[wave][i][l16][4 * g + r] = acc[i][r];      // [row][column]
+    __syncthreads();
+    auto finish = [&](auto tag) __attribute__((always_inline)) {
+        typedef decltype(tag) OT;
+        for (int t = threadIdx.x; t < MQ * 256; t += blockDim.x) {
+            const int q = t >> 4, p = p0 + (t & 15);
+            if (q >= a.nq || p >= a.np) continue;
+            float v = 0.f;
+            for (int w = 0; w < waves; w++) v += sums[w][q >> 4][q & 15][t & 15];
+            const float b = a.bias != nullptr ? (float)reinterpret_cast<const OT*>(a.bias)[p] : 0.f;
+            if constexpr (DT == FWA2_E4M3) v = v * (a.q_scale[q] * a.p_scale[p]) + b;
+            else v += b;
+            asm("" : "+v"(v));
+            const int64_t at = (int64_t)q * a.np + p;
+            if (a.z != nullptr) reinterpret_cast<OT*>(a.z)[at] = (OT)v;
+            v = act_of(v, a.act);
+            asm("" : "+v"(v));
+            if (a.residual != nullptr) v += (float)reinterpret_cast<const OT*>(a.residual + q * a.residual_stride)[p];
+            asm("" : "+v"(v));
+            reinterpret_cast<OT*>(a.out)[at] = (OT)v;
+        }
+    };
+    if constexpr (DT == FWA2_E4M3) {
+        if (a.out_bf16) finish((__bf16)0.f);
+        else finish((_Float16)0.f);
+    } else {
+        finish((typename Elem<DT == FWA2_E4M3 ? FWA2_F16 : DT>::E)0.f);
+    }
+}
+
 #if FWA2_HALF != 3
-// dW, db = sums of partial rows, rounded once.  A workgroup owns 256 values; its 16 wavefronts take every 16th partial (a
+// dW, db = sums of partial rows, rounded once.  A workgroup owns 256 values; its W wavefronts take every W-th partial (a
 // fixed assignment) and their sums are added in order.
-template <class E>
-__global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, int parts, const float* part_db, int parts_db,
+// (16 wavefronts for many partials, 4 for few.)
+template <class E, int W>
+__global__ void __launch_bounds__(64 * W) linear_sum_kernel(const float* part, int parts, const float* part_db, int parts_db,
                                                           int64_t cells, int64_t nq, E* out, E* db) {
-    __shared__ float s[16][256];
+    __shared__ float s[W][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t blocks = (cells + 255) / 256;
     const bool rows = blockIdx.x >= blocks;         // the workgroups behind those of dW sum db
@@ -739,17 +838,18 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, int
     if (n % 4 == 0) {
         if (i0 < n) {
 #pragma unroll 8
-            for (int k = wave; k < n_parts; k += 16) {
+            for (int k = wave; k < n_parts; k += W) {
                 const f32x4 v = *reinterpret_cast<const f32x4*>(src + (int64_t)k * n + i0);
 #pragma unroll
                 for (int j = 0; j < 4; j++) t[j] += v[j];
             }
         }
     } else {
-        for (int k = wave; k < n_parts; k += 16)
+        // (columns beyond the last repeat it, so that the loads need no branch)
+#pragma unroll 8
+        for (int k = wave; k < n_parts; k += W)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i0 + j < n) t[j] += src[(int64_t)k * n + i0 + j];
+            for (int j = 0; j < 4; j++) t[j] += src[(int64_t)k * n + (i0 + j < n ? i0 + j : n - 1)];
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) s[wave][4 * lane + j] = t[j];
@@ -758,7 +858,7 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, int
         const int64_t i = i0 - 4 * lane + threadIdx.x;
         if (i < n) {
             float v = 0.f;
-            for (int k = 0; k < 16; k++) v += s[k][threadIdx.x];
+            for (int k = 0; k < W; k++) v += s[k][threadIdx.x];
             (rows ? db : out)[i] = (E)v;
         }
     }
@@ -767,7 +867,7 @@ __global__ void __launch_bounds__(1024) linear_sum_kernel(const float* part, int
 // dz = dy act'(z), contiguous, and the column sums of dz before its rounding (part_db, one partial row per blockIdx.y).
 // A workgroup owns up to 512 columns (8 per lane, `lanes` lanes a row, a power of two) and a stretch of rows; bound by its
 // three streams.
-constexpr int kActRows = 1024;      // at most so many stretches of rows: their partial sums stay small
+constexpr int kActRows = 256;      // at most so many stretches of rows: their partial sums stay small
 template <class E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t dy_stride, const E* z, E* dz, int64_t rows,
                                                            int n, int lanes, int64_t rows_per_block, float* part_db, int act) {
@@ -830,7 +930,7 @@ static ActPlan plan_act(int64_t rows, int n, int cus) {
     pl.blocks_x = (chunks + pl.lanes - 1) / pl.lanes;
     int64_t y = (8 * (int64_t)cus + pl.blocks_x - 1) / pl.blocks_x;
     if (y > kActRows) y = kActRows;
-    const int64_t step = 256 / pl.lanes, most = (rows + step - 1) / step;
+    const int64_t step = 4 * (256 / pl.lanes), most = (rows + step - 1) / step;     // at least 4 rows per lane
     if (y > most) y = most;
     pl.rows_per_block = (rows + y - 1) / y;
     pl.blocks_y = (int)((rows + pl.rows_per_block - 1) / pl.rows_per_block);
@@ -945,22 +1045,44 @@ static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t s
 #undef FWA2_GO
 }
 
+// Up to 64 rows take the kernel made for them, whatever the other sizes.
+template <int DT>
+static void launch_rows(const LinArgs& a, hipStream_t st) {
+    const int64_t steps = (a.nk * LinElem<DT>::bytes + Frag16<DT>::BYTES - 1) / Frag16<DT>::BYTES;
+    int waves = kRowsWaves;
+    while (waves > 4 && waves > steps) waves /= 2;
+    const dim3 grid((a.np + 15) / 16), block(64 * waves);
+    if (a.nq <= 16) hipLaunchKernelGGL((linear_rows_kernel<DT, 1>), grid, block, 0, st, a);
+    else if (a.nq <= 32) hipLaunchKernelGGL((linear_rows_kernel<DT, 2>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((linear_rows_kernel<DT, 4>), grid, block, 0, st, a);
+}
+
 // The activations a product is compiled for; the others are decided at run time, row by row of the epilogue.
 template <int DT>
 static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, hipStream_t st) {
+    if (vec && a.nq <= kRowsMax) {
+        launch_rows<DT>(a, st);
+        return;
+    }
     if (a.act == FWA2_ACT_NONE) launch_product<DT, false, false, FWA2_ACT_NONE>(a, pl, vec, st);
     else if (a.act == FWA2_ACT_GELU) launch_product<DT, false, false, FWA2_ACT_GELU>(a, pl, vec, st);
     else launch_product<DT, false, false, -1>(a, pl, vec, st);
 }
 
-// Tiles for operands that go through registers.
+// Tiles for operands that go through registers: 128 wide when those fill the chip twice (their loads are waited for stage by
+// stage, so there have to be several workgroups to a CU), 64 otherwise.
 static LinPlan plan_unaligned(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
-    LinPlan pl = plan_product(nq, np, nk, split, elem_bytes, cus);
-    const int b = pl.tile == T64 ? 64 : 128;
-    pl.tile = b == 64 ? T64 : T128S;
+    LinPlan pl;
+    auto count = [&](int b) { return ((nq + b - 1) / b) * ((np + b - 1) / b); };
+    pl.tile = count(128) >= 2 * cus ? T128S : T64;
+    const int b = kTiles[pl.tile].bp;
     pl.tiles_p = (np + b - 1) / b;
-    pl.tiles = (nq + b - 1) / b * pl.tiles_p;
-    const int64_t ke = 64 / elem_bytes, stages = (nk + ke - 1) / ke, per = (stages + pl.splits - 1) / pl.splits;
+    pl.tiles = count(b);
+    const int64_t ke = 64 / elem_bytes, stages = (nk + ke - 1) / ke;
+    int64_t s = split ? 4 * (int64_t)cus / pl.tiles : 1;
+    if (s > stages / 4) s = stages / 4;
+    if (s < 1) s = 1;
+    const int64_t per = (stages + s - 1) / s;
     pl.k_per_split = per * ke;
     pl.splits = (int)((stages + per - 1) / per);
     return pl;
@@ -1067,9 +1189,13 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         const bool sum_db = p->dbias != nullptr && (part_act || pl.splits > 1);
         if (summed || sum_db) {
             const int64_t blocks = (summed + 255) / 256 + (sum_db ? (n + 255) / 256 : 0);
-            hipLaunchKernelGGL(linear_sum_kernel<E>, dim3((unsigned)blocks), dim3(1024), 0, st, a.part, pl.splits,
-                               part_act ? part_act : a.part_db, part_act ? act.blocks_y : pl.splits, summed, (int64_t)n,
-                               reinterpret_cast<E*>(p->dweight), reinterpret_cast<E*>(p->dbias));
+            const float* part_db = part_act ? part_act : a.part_db;
+            const int parts_db = part_act ? act.blocks_y : pl.splits;
+            E *dw = reinterpret_cast<E*>(p->dweight), *db = reinterpret_cast<E*>(p->dbias);
+            if (pl.splits > 32 || !summed)
+                hipLaunchKernelGGL((linear_sum_kernel<E, 16>), dim3((unsigned)blocks), dim3(1024), 0, st, a.part, pl.splits, part_db, parts_db, summed, (int64_t)n, dw, db);
+            else
+                hipLaunchKernelGGL((linear_sum_kernel<E, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a.part, pl.splits, part_db, parts_db, summed, (int64_t)n, dw, db);
         }
     }
 }
