@@ -730,22 +730,23 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
 template <int DT> struct Frag16 {           // v_mfma_f32_16x16x32
     typedef typename Elem<DT>::V8 V;
     static constexpr int BYTES = 64;        // of a row per product
-    static __device__ __forceinline__ V load(const char* row, int64_t left, int g) {
-        if (16 * g < left) return *reinterpret_cast<const V*>(row + 16 * g);
-        return zero8<V>();
+    static __device__ __forceinline__ V load(const char* row, int64_t at, int64_t left, int g) {
+        // beyond the end: the start of the row is read and zeros are used (a select, where a branch would wait)
+        const V v = *reinterpret_cast<const V*>(row + (16 * g < left ? at + 16 * g : 0));
+        return 16 * g < left ? v : zero8<V>();
     }
     static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) { return Elem<DT>::mfma16(a, b, c); }
 };
 template <> struct Frag16<FWA2_E4M3> {      // v_mfma_f32_16x16x128
     typedef i32x8 V;
     static constexpr int BYTES = 128;
-    static __device__ __forceinline__ V load(const char* row, int64_t left, int g) {
-        u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-        if (16 * g < left) a = *reinterpret_cast<const u32x4*>(row + 16 * g);
-        if (64 + 16 * g < left) b = *reinterpret_cast<const u32x4*>(row + 64 + 16 * g);
+    static __device__ __forceinline__ V load(const char* row, int64_t at, int64_t left, int g) {
+        const bool in_a = 16 * g < left, in_b = 64 + 16 * g < left;
+        const u32x4 a = *reinterpret_cast<const u32x4*>(row + (in_a ? at + 16 * g : 0));
+        const u32x4 b = *reinterpret_cast<const u32x4*>(row + (in_b ? at + 64 + 16 * g : 0));
         V v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) { v[i] = (int)a[i]; v[4 + i] = (int)b[i]; }
+        for (int i = 0; i < 4; i++) { v[i] = in_a ? (int)a[i] : 0; v[4 + i] = in_b ? (int)b[i] : 0; }
         return v;
     }
     static __device__ __forceinline__ f32x4 mfma(V a, V b, f32x4 c) {
@@ -769,6 +770,22 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
     f32x4 acc[MQ];
 #pragma unroll
     for (int i = 0; i < MQ; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // what the epilogue needs besides the sums is asked for first: value t of this thread is (row, column)
+    // (t / 16, t % 16) of the workgroup's, t = threadIdx.x + k blockDim.x with at least 256 threads
+    typedef typename std::conditional<DT == FWA2_E4M3, uint16_t, typename Elem<DT == FWA2_E4M3 ? FWA2_F16 : DT>::E>::type RT;
+    RT bias = {}, res[MQ];
+    float p_scale = 1.f, q_scale[MQ];
+    const int p = min(p0 + (int)(threadIdx.x & 15), a.np - 1);
+    if (a.bias != nullptr) bias = reinterpret_cast<const RT*>(a.bias)[p];
+    if (DT == FWA2_E4M3) p_scale = a.p_scale[p];
+#pragma unroll
+    for (int k = 0; k < MQ; k++) {
+        const int q = min((int)(threadIdx.x + k * blockDim.x) >> 4, (int)a.nq - 1);
+        res[k] = {};
+        q_scale[k] = 1.f;
+        if (a.residual != nullptr) res[k] = reinterpret_cast<const RT*>(a.residual + q * a.residual_stride)[p];
+        if (DT == FWA2_E4M3) q_scale[k] = a.q_scale[q];
+    }
     const int64_t bytes = a.nk * EB;
     const int64_t steps = (bytes + F::BYTES - 1) / F::BYTES;
     // every `waves`-th product is this wavefront's: neighbouring wavefronts read neighbouring stretches
@@ -777,9 +794,9 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t at = (s + (int64_t)u * waves) * F::BYTES;     // beyond the end: zeros
-            fp[u] = F::load(prow + at, bytes - at, g);
+            fp[u] = F::load(prow, at, bytes - at, g);
 #pragma unroll
-            for (int i = 0; i < MQ; i++) fq[u][i] = F::load(qrow[i] + at, bytes - at, g);
+            for (int i = 0; i < MQ; i++) fq[u][i] = F::load(qrow[i], at, bytes - at, g);
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -793,20 +810,21 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
     __syncthreads();
     auto finish = [&](auto tag) __attribute__((always_inline)) {
         typedef decltype(tag) OT;
-        for (int t = threadIdx.x; t < MQ * 256; t += blockDim.x) {
-            const int q = t >> 4, p = p0 + (t & 15);
-            if (q >= a.nq || p >= a.np) continue;
+#pragma unroll
+        for (int k = 0; k < MQ; k++) {
+            const int t = threadIdx.x + k * blockDim.x, q = t >> 4;
+            if (t >= MQ * 256 || q >= a.nq || p0 + (t & 15) >= a.np) continue;
             float v = 0.f;
             for (int w = 0; w < waves; w++) v += sums[w][q >> 4][q & 15][t & 15];
-            const float b = a.bias != nullptr ? (float)reinterpret_cast<const OT*>(a.bias)[p] : 0.f;
-            if constexpr (DT == FWA2_E4M3) v = v * (a.q_scale[q] * a.p_scale[p]) + b;
+            const float b = (float)__builtin_bit_cast(OT, bias);
+            if constexpr (DT == FWA2_E4M3) v = v * (q_scale[k] * p_scale) + b;
             else v += b;
             asm("" : "+v"(v));
             const int64_t at = (int64_t)q * a.np + p;
             if (a.z != nullptr) reinterpret_cast<OT*>(a.z)[at] = (OT)v;
             v = act_of(v, a.act);
             asm("" : "+v"(v));
-            if (a.residual != nullptr) v += (float)reinterpret_cast<const OT*>(a.residual + q * a.residual_stride)[p];
+            if (a.residual != nullptr) v += (float)__builtin_bit_cast(OT, res[k]);
             asm("" : "+v"(v));
             reinterpret_cast<OT*>(a.out)[at] = (OT)v;
         }
@@ -820,46 +838,57 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
 }
 
 #if FWA2_HALF != 3
-// dW, db = sums of partial rows, rounded once.  A workgroup owns 256 values; its W wavefronts take every W-th partial (a
-// fixed assignment) and their sums are added in order.
+// dW, db = sums of partial rows, rounded once.  A workgroup owns 256 values of dW (64 of db: there are few and each has many
+// partials); its W wavefronts take every W-th partial (a fixed assignment) and their sums are added in order.
 // (16 wavefronts for many partials, 4 for few.)
 template <class E, int W>
 __global__ void __launch_bounds__(64 * W) linear_sum_kernel(const float* part, int parts, const float* part_db, int parts_db,
-                                                          int64_t cells, int64_t nq, E* out, E* db) {
+                                                          int64_t cells, int nq, E* out, E* db) {
     __shared__ float s[W][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t blocks = (cells + 255) / 256;
-    const bool rows = blockIdx.x >= blocks;         // the workgroups behind those of dW sum db
-    const float* src = rows ? part_db : part;
-    const int n_parts = rows ? parts_db : parts;
-    const int64_t n = rows ? nq : cells;
-    const int64_t i0 = (rows ? blockIdx.x - blocks : (int64_t)blockIdx.x) * 256 + 4 * lane;
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-    if (n % 4 == 0) {
-        if (i0 < n) {
+    if (blockIdx.x >= blocks) {         // the workgroups behind those of dW sum db
+        const int i = (int)(blockIdx.x - blocks) * 64 + lane;
+        const float* src = part_db + min(i, nq - 1);
+        float t = 0.f;
 #pragma unroll 8
-            for (int k = wave; k < n_parts; k += W) {
-                const f32x4 v = *reinterpret_cast<const f32x4*>(src + (int64_t)k * n + i0);
+        for (int k = wave; k < parts_db; k += W) t += src[(int64_t)k * nq];
+        s[wave][lane] = t;
+        __syncthreads();
+        if (threadIdx.x < 64 && i < nq) {
+            t = 0.f;
+            for (int k = 0; k < W; k++) t += s[k][lane];
+            db[i] = (E)t;
+        }
+        return;
+    }
+    const int64_t i0 = (int64_t)blockIdx.x * 256 + 4 * lane;
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    if (cells % 4 == 0) {
+        if (i0 < cells) {
+#pragma unroll 8
+            for (int k = wave; k < parts; k += W) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)k * cells + i0);
 #pragma unroll
                 for (int j = 0; j < 4; j++) t[j] += v[j];
             }
         }
     } else {
-        // (columns beyond the last repeat it, so that the loads need no branch)
-#pragma unroll 8
-        for (int k = wave; k < n_parts; k += W)
+        // (values beyond the last repeat it, so that the loads need no branch)
+#pragma unroll 4
+        for (int k = wave; k < parts; k += W)
 #pragma unroll
-            for (int j = 0; j < 4; j++) t[j] += src[(int64_t)k * n + (i0 + j < n ? i0 + j : n - 1)];
+            for (int j = 0; j < 4; j++) t[j] += part[(int64_t)k * cells + (i0 + j < cells ? i0 + j : cells - 1)];
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) s[wave][4 * lane + j] = t[j];
     __syncthreads();
     if (threadIdx.x < 256) {
         const int64_t i = i0 - 4 * lane + threadIdx.x;
-        if (i < n) {
+        if (i < cells) {
             float v = 0.f;
             for (int k = 0; k < W; k++) v += s[k][threadIdx.x];
-            (rows ? db : out)[i] = (E)v;
+            out[i] = (E)v;
         }
     }
 }
@@ -870,7 +899,7 @@ __global__ void __launch_bounds__(64 * W) linear_sum_kernel(const float* part, i
 constexpr int kActRows = 256;      // at most so many stretches of rows: their partial sums stay small
 template <class E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t dy_stride, const E* z, E* dz, int64_t rows,
-                                                           int n, int lanes, int64_t rows_per_block, float* part_db, int act) {
+                                                           int n, int lanes, int64_t rows_per_block, float* part_db) {
     typedef E V8 __attribute__((ext_vector_type(8)));
     __shared__ float sums[256][9];
     const int cl = threadIdx.x % lanes, rl = threadIdx.x / lanes, step = 256 / lanes;
@@ -890,18 +919,31 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t 
                 V8 r;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    float d = (float)g[j] * slope_of((float)v[j], ACT >= 0 ? ACT : act);
+                    float d = (float)g[j] * slope_of((float)v[j], ACT);
                     t[j] += d;
                     r[j] = (E)d;
                 }
                 *reinterpret_cast<V8*>(o) = r;
             } else {
+                if (c + 8 <= n) {       // whole chunks in one access of whatever alignment the rows have
+                    V8 g, v, r;
+                    __builtin_memcpy(&g, a, 16);
+                    __builtin_memcpy(&v, b, 16);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (c + j >= n) continue;
-                    const float d = (float)a[j] * slope_of((float)b[j], ACT >= 0 ? ACT : act);
-                    t[j] += d;
-                    o[j] = (E)d;
+                    for (int j = 0; j < 8; j++) {
+                        const float d = (float)g[j] * slope_of((float)v[j], ACT);
+                        t[j] += d;
+                        r[j] = (E)d;
+                    }
+                    __builtin_memcpy(o, &r, 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (c + j >= n) continue;
+                        const float d = (float)a[j] * slope_of((float)b[j], ACT);
+                        t[j] += d;
+                        o[j] = (E)d;
+                    }
                 }
             }
         }
@@ -1149,12 +1191,16 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         const bool vec = rows16(p->dy, p->dy_stride, n, 2) && al16(p->z);
         const E *dy = reinterpret_cast<const E*>(p->dy), *z = reinterpret_cast<const E*>(p->z);
 #define FWA2_GO(ACT, VEC) hipLaunchKernelGGL((act_backward_kernel<E, ACT, VEC>), grid, block, 0, st, dy, p->dy_stride, z, \
-                                             reinterpret_cast<E*>(ws), m, n, act.lanes, act.rows_per_block, part_act, p->activation)
-        if (!vec) FWA2_GO(-1, false);
-        else if (p->activation == FWA2_ACT_GELU) FWA2_GO(FWA2_ACT_GELU, true);
-        else if (p->activation == FWA2_ACT_GELU_TANH) FWA2_GO(FWA2_ACT_GELU_TANH, true);
-        else if (p->activation == FWA2_ACT_SILU) FWA2_GO(FWA2_ACT_SILU, true);
-        else FWA2_GO(FWA2_ACT_RELU, true);
+                                             reinterpret_cast<E*>(ws), m, n, act.lanes, act.rows_per_block, part_act)
+        auto go = [&](auto aligned) {
+            constexpr bool VEC = decltype(aligned)::value;
+            if (p->activation == FWA2_ACT_GELU) FWA2_GO(FWA2_ACT_GELU, VEC);
+            else if (p->activation == FWA2_ACT_GELU_TANH) FWA2_GO(FWA2_ACT_GELU_TANH, VEC);
+            else if (p->activation == FWA2_ACT_SILU) FWA2_GO(FWA2_ACT_SILU, VEC);
+            else FWA2_GO(FWA2_ACT_RELU, VEC);
+        };
+        if (vec) go(std::true_type());
+        else go(std::false_type());
 #undef FWA2_GO
         dz = ws;
         dz_stride = n;
@@ -1188,14 +1234,14 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         const int64_t summed = pl.splits > 1 ? cells : 0;
         const bool sum_db = p->dbias != nullptr && (part_act || pl.splits > 1);
         if (summed || sum_db) {
-            const int64_t blocks = (summed + 255) / 256 + (sum_db ? (n + 255) / 256 : 0);
+            const int64_t blocks = (summed + 255) / 256 + (sum_db ? (n + 63) / 64 : 0);
             const float* part_db = part_act ? part_act : a.part_db;
             const int parts_db = part_act ? act.blocks_y : pl.splits;
             E *dw = reinterpret_cast<E*>(p->dweight), *db = reinterpret_cast<E*>(p->dbias);
             if (pl.splits > 32 || !summed)
-                hipLaunchKernelGGL((linear_sum_kernel<E, 16>), dim3((unsigned)blocks), dim3(1024), 0, st, a.part, pl.splits, part_db, parts_db, summed, (int64_t)n, dw, db);
+                hipLaunchKernelGGL((linear_sum_kernel<E, 16>), dim3((unsigned)blocks), dim3(1024), 0, st, a.part, pl.splits, part_db, parts_db, summed, n, dw, db);
             else
-                hipLaunchKernelGGL((linear_sum_kernel<E, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a.part, pl.splits, part_db, parts_db, summed, (int64_t)n, dw, db);
+                hipLaunchKernelGGL((linear_sum_kernel<E, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a.part, pl.splits, part_db, parts_db, summed, n, dw, db);
         }
     }
 }

@@ -37,7 +37,7 @@ struct NormArgs {
     void *dx, *ds;
     float* part;                    // [workgroups][2][dim]
     int64_t rows;
-    uint32_t rows_per_gate;
+    uint32_t rows_per_gate, gates;
     int dim;
     float eps;
     int layer, pre, param_f32, gate_f32, want_params;
@@ -80,28 +80,55 @@ __device__ __forceinline__ void row_store8(T* row, int c0, int dim, const float*
             if (c0 + j < dim) row[c0 + j] = v[j];
     }
 }
-// weight, bias: element type decided at run time (read once per workgroup)
-__device__ __forceinline__ void param_load8(const void* p, bool f32, int dt, int c0, int dim, float* x) {
+// weight, bias: element type decided at run time, read once per workgroup; zeros beyond the last column.  Loads from clamped
+// places and selects, no branch per value: a branch would wait for each load before the next one is asked for.
+template <bool VEC, class T>
+__device__ __forceinline__ void param_read8(const T* p, int c0, int dim, float* x) {
+    if (VEC) {
+        const typename Vec8<T>::V v = *reinterpret_cast<const typename Vec8<T>::V*>(p + min(c0, dim - 8));
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        x[j] = 0.f;
-        if (c0 + j >= dim) continue;
-        if (f32) x[j] = reinterpret_cast<const float*>(p)[c0 + j];
-        else if (dt == FWA2_BF16) x[j] = (float)reinterpret_cast<const __bf16*>(p)[c0 + j];
-        else x[j] = (float)reinterpret_cast<const _Float16*>(p)[c0 + j];
+        for (int j = 0; j < 8; j++) x[j] = c0 < dim ? (float)v[j] : 0.f;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float v = (float)p[min(c0 + j, dim - 1)];
+            x[j] = c0 + j < dim ? v : 0.f;
+        }
     }
 }
-template <class T> struct TypeCode;
-template <> struct TypeCode<__bf16> { static constexpr int v = FWA2_BF16; };
-template <> struct TypeCode<_Float16> { static constexpr int v = FWA2_F16; };
-template <> struct TypeCode<float> { static constexpr int v = FWA2_F32; };
-
-template <class XT>
-__device__ __forceinline__ float gate_of(const NormArgs& a, int64_t row) {
-    if (a.gate == nullptr) return 1.f;
-    const uint32_t i = (uint32_t)row / a.rows_per_gate;
-    return a.gate_f32 ? reinterpret_cast<const float*>(a.gate)[i] : (float)reinterpret_cast<const XT*>(a.gate)[i];
+template <bool VEC, class XT>
+__device__ __forceinline__ void param_load8(const void* p, bool f32, int c0, int dim, float* x) {
+    if (f32) param_read8<VEC>(reinterpret_cast<const float*>(p), c0, dim, x);
+    else param_read8<VEC>(reinterpret_cast<const XT*>(p), c0, dim, x);
 }
+// The gate of the rows a lane walks over: its index moves by whole samples and a remainder from row to row (a division per
+// row would cost more than the row's statistics).
+template <class XT>
+struct GateWalk {
+    uint32_t at, left, skip, more;      // sample, rows into it; what a step adds to both
+    __device__ __forceinline__ void init(const NormArgs& a, int64_t row, int64_t step) {
+        at = left = skip = more = 0;
+        if (a.gate == nullptr) return;
+        at = (uint32_t)row / a.rows_per_gate;
+        left = (uint32_t)row - at * a.rows_per_gate;
+        skip = (uint32_t)step / a.rows_per_gate;
+        more = (uint32_t)step - skip * a.rows_per_gate;
+    }
+    // (rows beyond the last: the last sample's gate)
+    __device__ __forceinline__ float get(const NormArgs& a) const {
+        if (a.gate == nullptr) return 1.f;
+        const uint32_t i = at < a.gates ? at : a.gates - 1;
+        return a.gate_f32 ? reinterpret_cast<const float*>(a.gate)[i] : (float)reinterpret_cast<const XT*>(a.gate)[i];
+    }
+    __device__ __forceinline__ void next(const NormArgs& a) {
+        at += skip;
+        left += more;
+        if (left >= a.rows_per_gate) {
+            left -= a.rows_per_gate;
+            at++;
+        }
+    }
+};
 
 // ---- sums and maxima over the LPR lanes of a row -----------------------------------------------------------
 template <int CTRL>
@@ -208,10 +235,10 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_fwd_kernel(const NormArg
 #pragma unroll
     for (int c = 0; c < CPL; c++) {
         const int c0 = 8 * (c * LPR + l);
-        param_load8(a.weight, a.param_f32, TypeCode<XT>::v, c0, dim, w[c]);
+        param_load8<VEC, XT>(a.weight, a.param_f32, c0, dim, w[c]);
 #pragma unroll
         for (int j = 0; j < 8; j++) b[c][j] = 0.f;
-        if (a.bias) param_load8(a.bias, a.param_f32, TypeCode<XT>::v, c0, dim, b[c]);
+        if (a.bias) param_load8<VEC, XT>(a.bias, a.param_f32, c0, dim, b[c]);
     }
 
     XV xr[CPL];
@@ -236,10 +263,13 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_fwd_kernel(const NormArg
     // makes the same number of rounds, which the exchanges and barriers inside need
     const int64_t last = a.rows - 1;
     fetch(row < last ? row : last);
+    GateWalk<XT> gate;
+    gate.init(a, row, step);
     for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += step, row += step) {
         const bool ok = row <= last;
         const int64_t rr = ok ? row : last;
-        const float g = gate_of<XT>(a, rr);
+        const float g = gate.get(a);
+        gate.next(a);
         float v[CPL][8], s[CPL][8];
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
@@ -272,24 +302,25 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_fwd_kernel(const NormArg
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
             const int c0 = 8 * (c * LPR + l);
+            float qc = 0.f;     // columns beyond the row's end hold 0 - m: left out, whole chunks at a time where rows have those
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float d = (VEC ? c0 < dim : c0 + j < dim) ? v[c][j] - m : 0.f;
+                const float d = VEC || c0 + j < dim ? v[c][j] - m : 0.f;
                 v[c][j] = d;
-                q += d * d;
+                qc += d * d;
             }
+            q += !VEC || c0 < dim ? qc : 0.f;
         }
-        const float r = 1.f / sqrtf(row_sum<LPR>(q, red, slot) * inv_dim + a.eps);
+        // one v_rsq_f32 (1 ulp) instead of a square root and a division (some 30 instructions); its argument is at least eps
+        const float r = __builtin_amdgcn_rsqf(row_sum<LPR>(q, red, slot) * inv_dim + a.eps);
         if (a.stats != nullptr && ok && l == 0) a.stats[rr] = make_float2(m, r);
 
-        uint32_t amax = 0;
 #pragma unroll
         for (int c = 0; c < CPL; c++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float n = v[c][j] * r * w[c][j] + b[c][j];
-                v[c][j] = pre ? n : s[c][j] + g * n;
-                amax = MaxU::of(amax, abs_bits(v[c][j]));
+                v[c][j] = __builtin_fmaf(v[c][j] * r, w[c][j], b[c][j]);
+                if (!pre) v[c][j] = __builtin_fmaf(g, v[c][j], s[c][j]);
             }
         }
         if (a.y != nullptr && ok) {
@@ -301,6 +332,12 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_fwd_kernel(const NormArg
             }
         }
         if (a.y8 != nullptr) {
+            uint32_t amax = 0;
+#pragma unroll
+            for (int c = 0; c < CPL; c++)
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    amax = MaxU::of(amax, (VEC ? 8 * (c * LPR + l) < dim : 8 * (c * LPR + l) + j < dim) ? abs_bits(v[c][j]) : 0);
             const RowScale sc = scale_of(row_reduce<MaxU, LPR>(amax, red, slot));
             if (ok) {
                 if (l == 0) a.y8_scale[rr] = sc.scale;
@@ -332,7 +369,7 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArg
     float w[CPL][8], dw[CPL][8], db[CPL][8];
 #pragma unroll
     for (int c = 0; c < CPL; c++) {
-        param_load8(a.weight, a.param_f32, TypeCode<XT>::v, 8 * (c * LPR + l), dim, w[c]);
+        param_load8<VEC, XT>(a.weight, a.param_f32, 8 * (c * LPR + l), dim, w[c]);
 #pragma unroll
         for (int j = 0; j < 8; j++) dw[c][j] = db[c][j] = 0.f;
     }
@@ -376,10 +413,22 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArg
     int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
     const int64_t last = a.rows - 1;
     fetch(row < last ? row : last);
+    GateWalk<XT> gate;
+    gate.init(a, row, step);
     for (int64_t base = (int64_t)blockIdx.x * RPB; base < a.rows; base += step, row += step) {
         const bool ok = row <= last;
         const int64_t rr = ok ? row : last;
-        const float g = gate_of<XT>(a, rr);
+        const float g = gate.get(a);
+        gate.next(a);
+        if (base + RPB > a.rows && !ok) {       // a row beyond the last: adds zeros to the column sums
+            st = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < CPL; c++) {
+                vr[c] = (VT)0.f;
+                yr[c] = (YT)0.f;
+                if (TWO) xr[TWO ? c : 0] = (XT)0.f;
+            }
+        }
         const float m = st.x, r = st.y;
         float v[CPL][8], t[CPL][8], up[PRE ? CPL : 1][8];
         float c1 = 0.f, c2 = 0.f;
@@ -390,8 +439,7 @@ __global__ void __launch_bounds__(norm_block(LPR)) norm_bwd_kernel(const NormArg
                 float src = (float)vr[c][j];
                 if (TWO) src += g * (float)xr[TWO ? c : 0][j];
                 const float vh = (src - m) * r;
-                // a copy of the last row adds nothing to the column sums
-                const float dn = ok ? (PRE ? (float)yr[c][j] : g * (float)yr[c][j]) : 0.f;
+                const float dn = PRE ? (float)yr[c][j] : g * (float)yr[c][j];
                 dw[c][j] += dn * vh;
                 db[c][j] += dn;
                 v[c][j] = vh;
@@ -603,7 +651,7 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float* part, in
     float t = 0.f;
     if (col < dim) {
         const float* p = part + (int64_t)which * dim + col;
-#pragma unroll 4
+#pragma unroll 16
         for (int i = wave; i < parts; i += 16) t += p[(int64_t)i * 2 * dim];
     }
     s[wave][lane] = t;
@@ -644,6 +692,7 @@ static NormArgs norm_args(const fwa2_norm* p) {
     a.part = reinterpret_cast<float*>(p->workspace);
     a.rows = p->rows;
     a.rows_per_gate = (uint32_t)(p->gate ? p->rows_per_gate : 1);
+    a.gates = (uint32_t)(p->gate ? p->rows / p->rows_per_gate : 1);
     a.dim = p->dim;
     a.eps = p->eps;
     a.layer = p->kind == FWA2_NORM_LAYER;
@@ -658,7 +707,8 @@ hipError_t launch_norm_forward(const fwa2_norm* p, int cus, hipStream_t st) {
     const NormArgs a = norm_args(p);
     // 16-byte accesses: whole chunks per row, every row on a 16-byte boundary (outputs are contiguous, 8-byte for y8)
     const bool vec = p->dim % 8 == 0 && al16(p->x) && p->x_stride % 8 == 0 &&
-                     (!p->shortcut || (al16(p->shortcut) && p->shortcut_stride % 8 == 0)) && al16(p->y) && al16(p->h) && al16(p->y8);
+                     (!p->shortcut || (al16(p->shortcut) && p->shortcut_stride % 8 == 0)) && al16(p->y) && al16(p->h) && al16(p->y8) &&
+                     al16(p->weight) && al16(p->bias);
     const bool s32 = p->stream_dtype == FWA2_F32;
     if (p->dtype == FWA2_BF16) norm_forward_bf16(a, s32, vec, cus, st);
     else if (p->dtype == FWA2_F16) norm_forward_f16(a, s32, vec, cus, st);
@@ -673,7 +723,7 @@ hipError_t launch_norm_backward(const fwa2_norm* p, int cus, hipStream_t st) {
     const bool vec = p->dim % 8 == 0 && (!pre || two ? al16(p->x) && p->x_stride % 8 == 0 : al16(p->h)) &&
                      (!two || (al16(p->shortcut) && p->shortcut_stride % 8 == 0)) &&
                      (!p->dy || (al16(p->dy) && p->dy_stride % 8 == 0)) && (!pre || !p->dh || (al16(p->dh) && p->dh_stride % 8 == 0)) &&
-                     al16(p->dx) && (!pre || al16(p->dshortcut));
+                     al16(p->dx) && (!pre || al16(p->dshortcut)) && al16(p->weight);
     const bool s32 = p->stream_dtype == FWA2_F32;
     const int blocks = norm_bwd_blocks(p->rows, p->dim, cus);
     if (p->dtype == FWA2_BF16) norm_backward_bf16(a, s32, vec, blocks, st);
