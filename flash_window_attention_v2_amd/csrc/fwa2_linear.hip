@@ -260,15 +260,18 @@ struct Operand {
             if (n >= CE) {
                 __builtin_memcpy(&r[i], src, 16);
             } else if (n > 0) {
-                for (int j = 0; j < CE; j++) {
-                    if (j >= n) break;
-                    uint32_t e;
-                    if (EB == 2) e = reinterpret_cast<const uint16_t*>(src)[j];
-                    else e = reinterpret_cast<const uint8_t*>(src)[j];
-                    const int bit = j * EB * 8;
+                // from clamped places: all loads under way at once, where a test per element would wait for each
+                uint32_t e[CE];
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
-                        if (x == bit / 32) r[i][x] |= e << (bit % 32);
+                for (int j = 0; j < CE; j++) {
+                    const int at_j = min(j, n - 1);
+                    if (EB == 2) e[j] = reinterpret_cast<const uint16_t*>(src)[at_j];
+                    else e[j] = reinterpret_cast<const uint8_t*>(src)[at_j];
+                }
+#pragma unroll
+                for (int j = 0; j < CE; j++) {
+                    const int bit = j * EB * 8;
+                    r[i][bit / 32] |= (j < n ? e[j] : 0u) << (bit % 32);
                 }
             }
         }
@@ -691,23 +694,32 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
                     const int n = a.np - p;
                     OT* out = reinterpret_cast<OT*>(a.out) + q * a.np + at;
                     OT* z = reinterpret_cast<OT*>(a.z) + q * a.np + at;
-                    if (a.z != nullptr) {
+                    V8 r, t;
+                    if (a.residual != nullptr) {
+                        const OT* res = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + res_at;
+                        if (n >= 8) __builtin_memcpy(&r, res, 16);
+                        else
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (j < n) z[j] = (OT)v[j];
+                            for (int j = 0; j < 8; j++) r[j] = res[min(j, n - 1)];
                     }
+                    auto store = [&](OT* to) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                        if (n >= 8) __builtin_memcpy(to, &t, 16);
+                        else
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                if (j < n) to[j] = t[j];
+                    };
+                    if (a.z != nullptr) store(z);
                     act8<ACT>(v, a.act);
                     settle8(v);
                     if (a.residual != nullptr) {
-                        const OT* res = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + res_at;
 #pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (j < n) v[j] += (float)res[j];
+                        for (int j = 0; j < 8; j++) v[j] += (float)r[j];
                     }
                     settle8(v);
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (j < n) out[j] = (OT)v[j];
+                    store(out);
                 }
                 asm volatile("" ::: "memory");
             }
@@ -925,25 +937,29 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t 
                 }
                 *reinterpret_cast<V8*>(o) = r;
             } else {
+                V8 g, v, r;
                 if (c + 8 <= n) {       // whole chunks in one access of whatever alignment the rows have
-                    V8 g, v, r;
                     __builtin_memcpy(&g, a, 16);
                     __builtin_memcpy(&v, b, 16);
+                } else {                // the last one element by element, from clamped places
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const float d = (float)g[j] * slope_of((float)v[j], ACT);
-                        t[j] += d;
-                        r[j] = (E)d;
+                        g[j] = a[min(j, n - 1 - c)];
+                        v[j] = b[min(j, n - 1 - c)];
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float d = (float)g[j] * slope_of((float)v[j], ACT);
+                    t[j] += d;
+                    r[j] = (E)d;
+                }
+                if (c + 8 <= n) {
                     __builtin_memcpy(o, &r, 16);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (c + j >= n) continue;
-                        const float d = (float)a[j] * slope_of((float)b[j], ACT);
-                        t[j] += d;
-                        o[j] = (E)d;
-                    }
+                    for (int j = 0; j < 8; j++)
+                        if (c + j < n) o[j] = r[j];
                 }
             }
         }

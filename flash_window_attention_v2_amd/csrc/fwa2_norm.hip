@@ -50,7 +50,8 @@ template <> struct Vec8<float> { typedef float V __attribute__((ext_vector_type(
 
 // 8 elements from column c0 on, zeros beyond the row's end.  VEC: rows start on 16-byte boundaries and dim is a multiple
 // of 8.  Otherwise a whole chunk is still one access of whatever alignment the row has, and only the chunk that
-// crosses the row's end goes element by element.
+// crosses the row's end goes element by element, from clamped places: eight loads under way at once, where a test per
+// element would wait for each.
 template <bool VEC, class T>
 __device__ __forceinline__ typename Vec8<T>::V row_load8(const T* row, int c0, int dim) {
     typename Vec8<T>::V v;
@@ -60,8 +61,11 @@ __device__ __forceinline__ typename Vec8<T>::V row_load8(const T* row, int c0, i
     } else if (c0 + 8 <= dim) {
         __builtin_memcpy(&v, row + c0, sizeof(v));
     } else {
+        T e[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = c0 + j < dim ? row[c0 + j] : (T)0.f;
+        for (int j = 0; j < 8; j++) e[j] = row[min(c0 + j, dim - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = c0 + j < dim ? e[j] : (T)0.f;
     }
     return v;
 }

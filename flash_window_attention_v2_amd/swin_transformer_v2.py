@@ -17,6 +17,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
+from .block_ops import (fused_linear_fp8_func, fused_linear_func, quantize_rows_func, residual_norm_fp8_func,
+                        residual_norm_func)
 from .win_attention_func import (flash_win_attn_v2_func, flash_win_attn_v2_grid_func, flash_win_attn_v2_qkvpacked_func,
                                  win_attention_torch)
 from .flash_window_attention_v2 import CpbBias, MAPPED_MAX_N, tensor_version
@@ -57,7 +59,21 @@ def shifted_window_attn_mask(resolution, window_size, shift_size):
     return torch.where(tiles[:, None, :] != tiles[:, :, None], -100.0, 0.0)
 
 
+def _hooked(*modules):
+    """Whether any of the modules carries hooks, which a call around its forward would skip."""
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+
+
 class Mlp(nn.Module):
+    """fc1, activation, fc2.  With `is_fused` the products run on the library's kernels (the activation in the epilogue of
+    the first) wherever those apply: on the GPU in half precision, without active dropout, with an activation the library
+    knows.  With `fp8` both products of a call that records no gradient take 8-bit rows: weights quantised once per
+    version, activations row by row."""
+
+    is_fused = False
+    fp8 = False
+    _weights8 = None
+
     def __init__(self, in_features, hidden_features=None, out_features=None, act_layer=nn.GELU, drop=0.):
         super().__init__()
         self.fc1 = nn.Linear(in_features, hidden_features or in_features)
@@ -65,8 +81,68 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden_features or in_features, out_features or in_features)
         self.drop = nn.Dropout(drop)
 
+    def _activation(self):
+        """The library's name of the activation, or None."""
+        if type(self.act) is nn.GELU:
+            return "gelu" if self.act.approximate == "none" else "gelu_tanh"
+        return {nn.SiLU: "silu", nn.ReLU: "relu"}.get(type(self.act))
+
+    def fused_dtype(self, x):
+        """The dtype the fused products would run in for `x`, or None where they do not apply."""
+        if not (self.is_fused and x.is_cuda and self._activation()):
+            return None
+        if type(self.fc1) is not nn.Linear or type(self.fc2) is not nn.Linear or (self.training and self.drop.p > 0):
+            return None
+        if _hooked(self.fc1, self.act, self.fc2, self.drop):
+            return None
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else x.dtype
+        if dtype not in (torch.float16, torch.bfloat16):
+            return None
+        params = [p for m in (self.fc1, self.fc2) for p in (m.weight, m.bias) if p is not None]
+        if not torch.is_autocast_enabled() and any(p.dtype != dtype for p in params):
+            return None
+        return dtype
+
+    def fp8_ready(self, x):
+        """Whether a call with `x` takes the 8-bit products."""
+        if not self.fp8 or self.fused_dtype(x) is None:
+            return False
+        if self.fc1.in_features > 16384 or self.fc2.in_features > 16384:
+            return False
+        return not (torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())))
+
+    def weights8(self):
+        """((fc1 weight, scale), (fc2 weight, scale)) in 8 bits, kept until a weight changes (tensors that track no
+        modifications, as those made under torch.inference_mode, are quantised on every call)."""
+        ws = (self.fc1.weight, self.fc2.weight)
+        key = tuple((tensor_version(w), w.data_ptr(), w.dtype, w.device) for w in ws)
+        held = self._weights8
+        if held is not None and held[0] == key and all(k[0] is not None for k in key):
+            return held[1]
+        with torch.no_grad():
+            made = tuple(quantize_rows_func(w) for w in ws)
+        if not torch.cuda.is_current_stream_capturing():
+            self._weights8 = (key, made)
+        return made
+
+    def forward_fp8(self, x8, scale, dtype):
+        """The MLP over 8-bit rows (`residual_norm_fp8_func` or `quantize_rows_func` made them), result in `dtype`."""
+        (w1, s1), (w2, s2) = self.weights8()
+        b1, b2 = (None if m.bias is None else m.bias.detach().to(dtype) for m in (self.fc1, self.fc2))
+        h = fused_linear_fp8_func(x8, scale, w1, s1, b1, self._activation(), out_dtype=dtype)
+        h8, sh = quantize_rows_func(h)
+        return fused_linear_fp8_func(h8, sh, w2, s2, b2, out_dtype=dtype)
+
     def forward(self, x):
-        return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
+        if self.fp8_ready(x):
+            return self.forward_fp8(*quantize_rows_func(x), self.fused_dtype(x))
+        dtype = self.fused_dtype(x)
+        if dtype is None:
+            return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
+        # under autocast the parameters are cast on the way in, as the framework's linear does
+        w1, b1, w2, b2 = (None if p is None else p.to(dtype) for m in (self.fc1, self.fc2) for p in (m.weight, m.bias))
+        h = fused_linear_func(x.to(dtype), w1, b1, self._activation())
+        return fused_linear_func(h, w2, b2)
 
 
 def trunc_normal_(tensor, mean=0., std=1., a=-2., b=2.):
@@ -277,8 +353,9 @@ class SwinTransformerBlock(nn.Module):
 
     def __init__(self, dim, input_resolution, num_heads, window_size=7, shift_size=0, is_flash=True, mlp_ratio=4.,
                  qkv_bias=True, drop=0., attn_drop=0., drop_path=0., act_layer=nn.GELU, norm_layer=nn.LayerNorm,
-                 pretrained_window_size=0):
+                 pretrained_window_size=0, is_fused=False, fp8_mlp=False):
         super().__init__()
+        self.is_fused = is_fused
         self.dim = dim
         self.input_resolution = input_resolution
         self.num_heads = num_heads
@@ -298,6 +375,7 @@ class SwinTransformerBlock(nn.Module):
         self.drop_path = DropPath(drop_path) if drop_path > 0. else nn.Identity()
         self.norm2 = norm_layer(dim)
         self.mlp = Mlp(in_features=dim, hidden_features=int(dim * mlp_ratio), act_layer=act_layer, drop=drop)
+        self.mlp.is_fused, self.mlp.fp8 = is_fused, is_fused and fp8_mlp
         mask = None
         if self.shift_size > 0:
             mask = shifted_window_attn_mask(input_resolution, self.window_size, self.shift_size)
@@ -326,6 +404,48 @@ class SwinTransformerBlock(nn.Module):
             self._attn_mask_flags = (key, flags)
         return flags
 
+    def _norm_fused(self, norm, x, shortcut):
+        """Whether shortcut + drop_path(norm(x)) runs as the library's one call, with the framework's types."""
+        if not (self.is_fused and type(norm) is nn.LayerNorm and norm.weight is not None and x.is_cuda):
+            return False
+        if type(self.drop_path) not in (DropPath, nn.Identity) or _hooked(norm, self.drop_path) or x.shape[-1] > 16384:
+            return False
+        if norm.normalized_shape != (x.shape[-1],) or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            return False
+        if shortcut.dtype not in (x.dtype, torch.float32) or norm.weight.dtype not in (x.dtype, torch.float32):
+            return False
+        # under autocast the framework's norm returns fp32, and with it the sum
+        return not torch.is_autocast_enabled() or shortcut.dtype == torch.float32
+
+    def _gate(self, x):
+        """Stochastic depth's factor per sample (0 or 1 / keep), or None; drawn as `drop_path` draws it."""
+        p = self.drop_path.drop_prob if isinstance(self.drop_path, DropPath) else 0.
+        if p == 0. or not self.training:
+            return None
+        keep = 1.0 - p
+        return x.new_empty((x.shape[0],) + (1,) * (x.dim() - 1)).bernoulli_(keep).float() / keep
+
+    def _add_norm(self, norm, x, shortcut):
+        """shortcut + drop_path(norm(x)): the residual post-normalisation of both halves of the block."""
+        if self._norm_fused(norm, x, shortcut):
+            return residual_norm_func(x, shortcut, norm.weight, norm.bias, norm.eps, gate=self._gate(x))
+        return shortcut + self.drop_path(norm(x))
+
+    def _second_half(self, x, shortcut):
+        """Everything behind the attention: x = shortcut + norm1(x), x + norm2(mlp(x))."""
+        n = self.norm1
+        recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
+                                                   (shortcut, getattr(n, "weight", None), getattr(n, "bias", None)))
+        if not recorded and self.mlp.fp8_ready(x) and self._norm_fused(n, x, shortcut) and not _hooked(self.mlp):
+            # the rows leave the first norm in 8 bits next to the stream
+            dtype = self.mlp.fused_dtype(x)
+            with torch.no_grad():
+                x, x8, scale = residual_norm_fp8_func(x, shortcut, n.weight, n.bias, n.eps, gate=self._gate(x))
+                y = self.mlp.forward_fp8(x8, scale, dtype)
+            return self._add_norm(self.norm2, y, x)
+        x = self._add_norm(self.norm1, x, shortcut)
+        return self._add_norm(self.norm2, self.mlp(x), x)
+
     def forward(self, x):
         h, w = self.input_resolution
         b, length, c = x.shape
@@ -335,8 +455,7 @@ class SwinTransformerBlock(nn.Module):
             # roll, window_partition, window_reverse and the roll back happen inside the kernels
             x = self.attn.forward_grid(x, (h, w), (self.shift_size, self.shift_size), mask=self.attn_mask,
                                        mask_flags=self.mask_flags())
-            x = shortcut + self.drop_path(self.norm1(x))
-            return x + self.drop_path(self.norm2(self.mlp(x)))
+            return self._second_half(x, shortcut)
         x = x.view(b, h, w, c)
         if self.shift_size > 0:
             x = torch.roll(x, shifts=(-self.shift_size, -self.shift_size), dims=(1, 2))
@@ -345,8 +464,7 @@ class SwinTransformerBlock(nn.Module):
         x = window_reverse(windows.view(-1, self.window_size, self.window_size, c), self.window_size, h, w)
         if self.shift_size > 0:
             x = torch.roll(x, shifts=(self.shift_size, self.shift_size), dims=(1, 2))
-        x = shortcut + self.drop_path(self.norm1(x.reshape(b, h * w, c)))
-        return x + self.drop_path(self.norm2(self.mlp(x)))
+        return self._second_half(x.reshape(b, h * w, c), shortcut)
 
     def flops(self):
         """The reference's count (swin_transformer_v2.py:453-465): two norms, the windows' attention, the MLP."""
@@ -392,7 +510,7 @@ class BasicLayer(nn.Module):
 
     def __init__(self, dim, input_resolution, depth, num_heads, window_size, is_flash=True, mlp_ratio=4.,
                  qkv_bias=True, drop=0., attn_drop=0., drop_path=0., norm_layer=nn.LayerNorm, downsample=None,
-                 use_checkpoint=False, pretrained_window_size=0):
+                 use_checkpoint=False, pretrained_window_size=0, is_fused=False, fp8_mlp=False):
         super().__init__()
         self.dim = dim
         self.input_resolution = input_resolution
@@ -404,7 +522,8 @@ class BasicLayer(nn.Module):
                                  is_flash=is_flash, mlp_ratio=mlp_ratio, qkv_bias=qkv_bias, drop=drop,
                                  attn_drop=attn_drop,
                                  drop_path=drop_path[i] if isinstance(drop_path, (list, tuple)) else drop_path,
-                                 norm_layer=norm_layer, pretrained_window_size=pretrained_window_size)
+                                 norm_layer=norm_layer, pretrained_window_size=pretrained_window_size,
+                                 is_fused=is_fused, fp8_mlp=fp8_mlp)
             for i in range(depth)])
         self.downsample = downsample(input_resolution, dim=dim, norm_layer=norm_layer) if downsample else None
 
@@ -454,12 +573,14 @@ class PatchEmbed(nn.Module):
 
 class SwinTransformerV2(nn.Module):
     """Hierarchical Swin V2 classifier with the reference's constructor arguments and parameter
-    names (swin_transformer_v2.py:668-822)."""
+    names (swin_transformer_v2.py:668-822).  Two arguments go beyond it: `is_fused` runs the MLPs and the residual
+    post-normalisations of the blocks on the library's kernels (fewer roundings, so results differ in the last bits; off by
+    default), `fp8_mlp` with it the MLPs of calls that record no gradient on 8-bit rows."""
 
     def __init__(self, img_size=256, patch_size=4, in_chans=3, num_classes=1000, embed_dim=96, depths=[2, 2, 6, 2],
                  num_heads=[3, 6, 12, 24], window_size=8, is_flash=True, mlp_ratio=4., qkv_bias=True, drop_rate=0.,
                  attn_drop_rate=0., drop_path_rate=0.1, norm_layer=nn.LayerNorm, ape=False, patch_norm=True,
-                 use_checkpoint=False, pretrained_window_sizes=[0, 0, 0, 0], **kwargs):
+                 use_checkpoint=False, pretrained_window_sizes=[0, 0, 0, 0], is_fused=False, fp8_mlp=False, **kwargs):
         super().__init__()
         self.num_classes = num_classes
         self.num_layers = len(depths)
@@ -488,7 +609,8 @@ class SwinTransformerV2(nn.Module):
                 num_heads=num_heads[i], window_size=window_size, is_flash=is_flash, mlp_ratio=mlp_ratio,
                 qkv_bias=qkv_bias, drop=drop_rate, attn_drop=attn_drop_rate, drop_path=rates[first:first + depth],
                 norm_layer=norm_layer, downsample=PatchMerging if i < self.num_layers - 1 else None,
-                use_checkpoint=use_checkpoint, pretrained_window_size=pretrained_window_sizes[i]))
+                use_checkpoint=use_checkpoint, pretrained_window_size=pretrained_window_sizes[i], is_fused=is_fused,
+                fp8_mlp=fp8_mlp))
 
         self.norm = norm_layer(self.num_features)
         self.avgpool = nn.AdaptiveAvgPool1d(1)
