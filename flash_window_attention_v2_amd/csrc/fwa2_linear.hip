@@ -50,6 +50,7 @@ struct LinArgs {
     const float *q_scale, *p_scale;
     int act;
     int out_vec;                  // output rows (and residual, z, bias) take 16-byte accesses
+    int stream_out;               // non-temporal stores (stream_results)
     int out_bf16;                 // 8-bit products: element type of the output
 };
 
@@ -368,6 +369,147 @@ __device__ __forceinline__ int result_chunk(int q, int c) {
     return q * (TP / 4) + (c ^ x);
 }
 
+// The results of a wavefront: acc (rows of 32, 4 consecutive columns of 32 different rows per lane) changes hands through
+// `mine` (32 x TP floats of LDS that only this wavefront uses), so that TP / 8 neighbouring lanes hold whole stretches of a
+// row, and residual, z and result move in full cache lines: stored as they are, 32 rows would get 32 bytes each.
+template <int TP>
+struct Results {
+    static constexpr int LPR = TP / 8;             // lanes of a row
+    static constexpr int RPI = 64 / LPR;           // rows per instruction (TP = 96: 5, and four lanes idle)
+    static constexpr int NR = (32 + RPI - 1) / RPI;
+    char* mine;
+    int l32, half, rl, cl;
+
+    __device__ __forceinline__ void init(char* m, int lane) {
+        mine = m;
+        l32 = lane & 31;
+        half = lane >> 5;
+        rl = lane / LPR;
+        cl = lane - rl * LPR;
+    }
+    template <int FP>
+    __device__ __forceinline__ void put(const f32x16 (&acc)[FP]) const {
+#pragma unroll
+        for (int j = 0; j < FP; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const f32x4 v = {acc[j][4 * r], acc[j][4 * r + 1], acc[j][4 * r + 2], acc[j][4 * r + 3]};
+                *reinterpret_cast<f32x4*>(mine + 16 * result_chunk<TP>(l32, 8 * j + 2 * r + half)) = v;
+            }
+        asm volatile("" ::: "memory");      // a wavefront's LDS accesses stay in order
+    }
+    __device__ __forceinline__ void get(int row, float* v) const {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl));
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl + 1));
+#pragma unroll
+        for (int e = 0; e < 4; e++) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+    }
+};
+
+// bias, and before it the scales of an 8-bit product
+template <int DT, class OT>
+struct Columns {
+    float bias[8], ps[8];
+    __device__ __forceinline__ void init(const LinArgs& a, int p) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) bias[e] = 0.f;
+        if (a.bias != nullptr) load_bias<OT, 8>(a, p, bias);
+        if constexpr (DT == FWA2_E4M3) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) ps[e] = a.p_scale[min(p + e, a.np - 1)];
+        }
+    }
+    __device__ __forceinline__ void apply(const LinArgs& a, float* v, int64_t q) const {
+        if constexpr (DT == FWA2_E4M3) {
+            const float qs = a.q_scale[q];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = v[e] * (qs * ps[e]) + bias[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += bias[e];
+        }
+    }
+};
+
+// Epilogue of a wavefront's TQ x TP block with its first row at qw, first column at pw; output rows take 16-byte accesses (np
+// is a multiple of 8: a lane's 8 columns are inside or outside together).
+// Buffer accesses: rows beyond the last lie outside the buffer's size, lanes outside the columns are sent there, and the
+// hardware drops such stores and returns zeros for such loads; no branches, and all rows in one stretch of code.  A
+// wavefront's rows span less than 2^31 bytes (row strides are below 2^22 elements).
+template <int DT, class OT, int TP, int TQ, int ACT, int FQ, int FP>
+__device__ __forceinline__ void store_results(const LinArgs& a, const Results<TP>& r, f32x16 (&acc)[FQ][FP], int64_t qw, int pw) {
+    typedef OT V8 __attribute__((ext_vector_type(8)));
+    constexpr int RPI = Results<TP>::RPI, NR = Results<TP>::NR;
+    const int p = pw + 8 * r.cl;
+    const bool inside = r.rl < RPI && p < a.np;
+    Columns<DT, OT> columns;
+    columns.init(a, p);
+    const int rows = a.nq - qw < TQ ? (int)(a.nq - qw) : TQ;
+    const bool any = rows > 0;
+    auto buffer = [&](const void* base, int64_t row_bytes) __attribute__((always_inline)) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(uniform_pointer(reinterpret_cast<const char*>(base) + qw * row_bytes)), 0,
+                                                 any ? (int)(rows * row_bytes) : 0, 0x00027000);
+    };
+    const auto out_rows = buffer(a.out, (int64_t)a.np * 2);
+    const uint32_t out_step = (uint32_t)a.np * 2, res_step = (uint32_t)a.residual_stride;
+    const uint32_t out_at = inside ? (uint32_t)r.rl * out_step + (uint32_t)p * 2 : 0x80000000u;
+    const uint32_t from = inside ? (uint32_t)r.rl * res_step + (uint32_t)p * 2 : 0x80000000u;
+    auto body = [&](auto has_residual, auto has_z, auto stream) __attribute__((always_inline)) {
+        constexpr int policy = decltype(stream)::value ? kStreamPolicy : 0;
+        const auto res_rows = buffer(a.residual, has_residual ? a.residual_stride : 0);
+        const auto z_rows = buffer(a.z, has_z ? (int64_t)a.np * 2 : 0);
+#pragma unroll
+        for (int i = 0; i < FQ; i++) {
+            u32x4 res[NR];
+            if (has_residual) {
+#pragma unroll
+                for (int k = 0; k < NR; k++)
+                    res[k] = __builtin_amdgcn_raw_buffer_load_b128(res_rows, from + (32 * i + k * RPI) * res_step, 0, 0);
+            }
+            r.put(acc[i]);
+#pragma unroll
+            for (int k = 0; k < NR; k++) {
+                const uint32_t skip = 32 % RPI != 0 && k * RPI + r.rl >= 32 ? 0x80000000u : 0u;
+                float v[8];
+                r.get(32 % RPI == 0 ? k * RPI + r.rl : min(k * RPI + r.rl, 31), v);
+                columns.apply(a, v, any ? qw + min(32 * i + k * RPI + r.rl, rows - 1) : 0);
+                settle8(v);
+                V8 t;
+                if (has_z) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), z_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, policy);
+                }
+                act8<ACT>(v, a.act);
+                settle8(v);
+                if (has_residual) {
+                    const V8 x = __builtin_bit_cast(V8, res[k]);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] += (float)x[j];
+                }
+                settle8(v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), out_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, policy);
+            }
+            asm volatile("" ::: "memory");
+        }
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    auto with_policy = [&](auto stream) __attribute__((always_inline)) {
+        if (a.residual != nullptr) {
+            if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(yes, yes, stream);
+            else body(yes, no, stream);
+        } else {
+            if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(no, yes, stream);
+            else body(no, no, stream);
+        }
+    };
+    if (a.stream_out) with_policy(yes);
+    else with_policy(no);
+}
+
 // ACT: the activation, or -1 where it is decided at run time.  WAVES: wavefronts per SIMD the registers are limited for.
 template <int DT, bool PT, bool QT, int BP, int BQ, int WP, int WQ, int KB, int STAGES, bool VEC, int ACT, int WAVES>
 __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinArgs a) {
@@ -534,51 +676,29 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
             }
         }
     }
-    // The accumulators hold 4 consecutive columns of 32 different rows: written like that, every store would touch 32 rows
-    // with 32 bytes each.  They change hands through LDS instead (each wavefront its own part, 32 rows at a time), so that
-    // TP / 8 neighbouring lanes hold whole stretches of a row, and residual, z and result move in full cache lines.
-    lds_barrier();          // nobody reads operands any more
-    char* mine = lds + wave * 32 * TP * 4;
-    constexpr int LPR = TP / 8;             // lanes of a row
-    constexpr int RPI = 64 / LPR;           // rows per instruction (TP = 96: 5, and four lanes idle)
-    const int rl = lane / LPR, cl = lane - rl * LPR;
-    const int p = p0 + wp * TP + 8 * cl;
-    const bool inside = rl < RPI && p < a.np;
+    lds_barrier();          // nobody reads operands any more: their memory takes the results
+    typedef Results<TP> RS;
+    RS r;
+    r.init(lds + wave * 32 * TP * 4, lane);
     const int64_t qw = q0 + wq * TQ;        // uniform: first row of this wavefront
-    auto put = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < FP; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const f32x4 v = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-                *reinterpret_cast<f32x4*>(mine + 16 * result_chunk<TP>(l32, 8 * j + 2 * r + half)) = v;
-            }
-        asm volatile("" ::: "memory");      // a wavefront's LDS accesses stay in order
-    };
-    auto get = [&](int row, float* v) __attribute__((always_inline)) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl));
-        const f32x4 hi = *reinterpret_cast<const f32x4*>(mine + 16 * result_chunk<TP>(row, 2 * cl + 1));
-#pragma unroll
-        for (int e = 0; e < 4; e++) { v[e] = lo[e]; v[4 + e] = hi[e]; }
-    };
+    const int pw = p0 + wp * TP, p = pw + 8 * r.cl;
     // Is row r0 + rl of the 32 this lane's business?  (q: the uniform part of its index in the output)
     auto mine_row = [&](int r0, int64_t q) __attribute__((always_inline)) {
-        return inside && (32 % RPI == 0 || r0 + rl < 32) && q + rl < a.nq;
+        return r.rl < RS::RPI && p < a.np && (32 % RS::RPI == 0 || r0 + r.rl < 32) && q + r.rl < a.nq;
     };
-    // uniform row pointers and a 32-bit offset per lane: no 64-bit address arithmetic on the vector unit
-    const uint32_t at = (uint32_t)rl * (uint32_t)a.np + (uint32_t)p;
+    const uint32_t at = (uint32_t)r.rl * (uint32_t)a.np + (uint32_t)p;
     if (a.splits > 1) {
         float* out = a.part + (int64_t)split * a.nq * a.np;
         const bool whole = a.np % 8 == 0;
 #pragma unroll
         for (int i = 0; i < FQ; i++) {
-            put(i);
+            r.put(acc[i]);
 #pragma unroll
-            for (int r0 = 0; r0 < 32; r0 += RPI) {
+            for (int r0 = 0; r0 < 32; r0 += RS::RPI) {
                 const int64_t q = qw + 32 * i + r0;
                 if (!mine_row(r0, q)) continue;
                 float v[8];
-                get(r0 + rl, v);
+                r.get(r0 + r.rl, v);
                 float* o = out + q * a.np + at;
                 if (whole) {
                     *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
@@ -596,133 +716,53 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
     auto finish = [&](auto tag) __attribute__((always_inline)) {
         typedef decltype(tag) OT;
         typedef OT V8 __attribute__((ext_vector_type(8)));
-        constexpr int NR = (32 + RPI - 1) / RPI;
-        float bias[8], ps[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) bias[e] = 0.f;
-        if (a.bias != nullptr) load_bias<OT, 8>(a, p, bias);
-        if constexpr (DT == FWA2_E4M3) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) ps[e] = a.p_scale[min(p + e, a.np - 1)];
+        if (a.out_vec) {
+            store_results<DT, OT, TP, TQ, ACT>(a, r, acc, qw, pw);
+            return;
         }
-        // bias, and before it the scales of an 8-bit product
-        auto scaled = [&](float* v, int64_t q) __attribute__((always_inline)) {
-            if constexpr (DT == FWA2_E4M3) {
-                const float qs = a.q_scale[q];
+        Columns<DT, OT> columns;
+        columns.init(a, p);
+        const uint32_t res_at = (uint32_t)r.rl * (uint32_t)(a.residual_stride / 2) + (uint32_t)p;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = v[e] * (qs * ps[e]) + bias[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) v[e] += bias[e];
-            }
-        };
-        const uint32_t res_at = (uint32_t)rl * (uint32_t)(a.residual_stride / 2) + (uint32_t)p;
-        if (a.out_vec) {        // np is a multiple of 8: a lane's 8 columns are inside or outside together
-            // Buffer accesses: rows beyond the last lie outside the buffer's size, lanes outside the columns are sent there,
-            // and the hardware drops such stores and returns zeros for such loads; no branches, and all rows in one
-            // stretch of code.  A wavefront's rows span less than 2^31 bytes (row strides are below 2^22 elements).
-            const int rows = a.nq - qw < TQ ? (int)(a.nq - qw) : TQ;
-            const bool any = rows > 0;
-            auto buffer = [&](const void* base, int64_t row_bytes) __attribute__((always_inline)) {
-                return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(uniform_pointer(reinterpret_cast<const char*>(base) + qw * row_bytes)), 0,
-                                                         any ? (int)(rows * row_bytes) : 0, 0x00027000);
-            };
-            const auto out_rows = buffer(a.out, (int64_t)a.np * 2);
-            const uint32_t out_at = inside ? at * 2 : 0x80000000u, out_step = (uint32_t)a.np * 2;
-            const uint32_t from = inside ? res_at * 2 : 0x80000000u, res_step = (uint32_t)a.residual_stride;
-            auto body = [&](auto has_residual, auto has_z) __attribute__((always_inline)) {
-                const auto res_rows = buffer(a.residual, has_residual ? a.residual_stride : 0);
-                const auto z_rows = buffer(a.z, has_z ? (int64_t)a.np * 2 : 0);
-#pragma unroll
-                for (int i = 0; i < FQ; i++) {
-                    u32x4 res[NR];
-                    if (has_residual) {
-#pragma unroll
-                        for (int k = 0; k < NR; k++)
-                            res[k] = __builtin_amdgcn_raw_buffer_load_b128(res_rows, from + (32 * i + k * RPI) * res_step, 0, 0);
-                    }
-                    put(i);
-#pragma unroll
-                    for (int k = 0; k < NR; k++) {
-                        const uint32_t skip = 32 % RPI != 0 && k * RPI + rl >= 32 ? 0x80000000u : 0u;
-                        float v[8];
-                        get(32 % RPI == 0 ? k * RPI + rl : min(k * RPI + rl, 31), v);
-                        scaled(v, any ? qw + min(32 * i + k * RPI + rl, rows - 1) : 0);
-                        settle8(v);
-                        V8 t;
-                        if (has_z) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), z_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, 0);
-                        }
-                        act8<ACT>(v, a.act);
-                        settle8(v);
-                        if (has_residual) {
-                            const V8 r = __builtin_bit_cast(V8, res[k]);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) v[j] += (float)r[j];
-                        }
-                        settle8(v);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, t), out_rows, (out_at | skip) + (32 * i + k * RPI) * out_step, 0, 0);
-                    }
-                    asm volatile("" ::: "memory");
-                }
-            };
-            const std::true_type yes;
-            const std::false_type no;
-            if (a.residual != nullptr) {
-                if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(yes, yes);
-                else body(yes, no);
-            } else {
-                if (ACT != FWA2_ACT_NONE && a.z != nullptr) body(no, yes);
-                else body(no, no);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < FQ; i++) {
-                put(i);
+        for (int i = 0; i < FQ; i++) {
+            r.put(acc[i]);
 #pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += RPI) {
-                    const int64_t q = qw + 32 * i + r0;
-                    if (!mine_row(r0, q)) continue;
-                    float v[8];
-                    get(r0 + rl, v);
-                    scaled(v, q + rl);
-                    settle8(v);
-                    const int n = a.np - p;
-                    OT* out = reinterpret_cast<OT*>(a.out) + q * a.np + at;
-                    OT* z = reinterpret_cast<OT*>(a.z) + q * a.np + at;
-                    V8 r, t;
-                    if (a.residual != nullptr) {
-                        const OT* res = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + res_at;
-                        if (n >= 8) __builtin_memcpy(&r, res, 16);
-                        else
+            for (int r0 = 0; r0 < 32; r0 += RS::RPI) {
+                const int64_t q = qw + 32 * i + r0;
+                if (!mine_row(r0, q)) continue;
+                float v[8];
+                r.get(r0 + r.rl, v);
+                columns.apply(a, v, q + r.rl);
+                settle8(v);
+                const int n = a.np - p;
+                V8 res, t;
+                if (a.residual != nullptr) {
+                    const OT* src = reinterpret_cast<const OT*>(a.residual + q * a.residual_stride) + res_at;
+                    if (n >= 8) __builtin_memcpy(&res, src, 16);
+                    else
 #pragma unroll
-                            for (int j = 0; j < 8; j++) r[j] = res[min(j, n - 1)];
-                    }
-                    auto store = [&](OT* to) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
-                        if (n >= 8) __builtin_memcpy(to, &t, 16);
-                        else
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                if (j < n) to[j] = t[j];
-                    };
-                    if (a.z != nullptr) store(z);
-                    act8<ACT>(v, a.act);
-                    settle8(v);
-                    if (a.residual != nullptr) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) v[j] += (float)r[j];
-                    }
-                    settle8(v);
-                    store(out);
+                        for (int j = 0; j < 8; j++) res[j] = src[min(j, n - 1)];
                 }
-                asm volatile("" ::: "memory");
+                auto store = [&](OT* to) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[j] = (OT)v[j];
+                    if (n >= 8) __builtin_memcpy(to, &t, 16);
+                    else
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (j < n) to[j] = t[j];
+                };
+                if (a.z != nullptr) store(reinterpret_cast<OT*>(a.z) + q * a.np + at);
+                act8<ACT>(v, a.act);
+                settle8(v);
+                if (a.residual != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] += (float)res[j];
+                }
+                settle8(v);
+                store(reinterpret_cast<OT*>(a.out) + q * a.np + at);
             }
+            asm volatile("" ::: "memory");
         }
     };
     if constexpr (DT == FWA2_E4M3) {
@@ -1043,7 +1083,7 @@ static LinPlan plan_product(int64_t nq, int np, int64_t nk, bool split, int elem
         pl.tile = T256;             // whole rounds of full tiles and a contraction that hides the ends
     } else if (split) {
         pl.tile = small ? T64 : wide(np) && np > 128 ? (wide(nq) && nq > 128 ? T192 : T192P) : (wide(nq) && nq > 128 ? T192Q : T128);
-    } else if (small || count(T128) < cus) {
+    } else if (small || count(T128) * 10 < 6 * cus) {
         pl.tile = T64;
     } else if (nk * elem_bytes <= 384) {
         pl.tile = T128S;
@@ -1155,6 +1195,13 @@ static inline bool rows16(const void* p, int64_t stride, int64_t len, int bytes)
     return al16(p) && stride * bytes % 16 == 0 && len * bytes % 16 == 0;
 }
 
+// Results too large to be found in the 256 MB memory-side cache by whoever reads them next leave with non-temporal stores: plain
+// ones fill the L2s with lines that wait to be written back, behind which the operands of the next tiles queue.  Measured
+// (us, plain / non-temporal): 262144 x 96 -> 384 with GELU 90 / 65, without 80 / 45; 65536 x 192 -> 768 46 / 32;
+// 16384 x 384 -> 1536 with z 44 / 38.  An MLP whose second product reads the 201 MB of the first: 178 / 184 forward, but
+// 804 / 762 forward and backward.  Smaller results stay in the cache: 100 MB and less gained nothing in such a chain.
+static bool stream_results(int64_t rows, int columns, bool z) { return (double)rows * columns * (z ? 4 : 2) >= (64 << 20); }
+
 static LinArgs forward_args(const fwa2_linear* p) {
     const int xb = p->x_dtype == FWA2_E4M3 ? 1 : 2;
     LinArgs a = {};
@@ -1165,6 +1212,7 @@ static LinArgs forward_args(const fwa2_linear* p) {
     a.residual = reinterpret_cast<const char*>(p->residual); a.residual_stride = p->residual_stride * 2;
     a.q_scale = p->x_scale; a.p_scale = p->weight_scale;
     a.out_bf16 = p->dtype == FWA2_BF16;
+    a.stream_out = stream_results(p->rows, p->out_features, p->z != nullptr);
     a.out_vec = p->out_features % 8 == 0 && al16(p->y) && al16(p->z) && al16(p->bias) && (!p->residual || rows16(p->residual, p->residual_stride, 8, 2));
     return a;
 }
@@ -1229,6 +1277,7 @@ void FWA2_LIN_FN(linear_backward)(const fwa2_linear* p, int cus, hipStream_t st)
         a.p = reinterpret_cast<const char*>(p->weight); a.p_stride = p->weight_stride * 2;
         a.nq = m; a.np = k; a.nk = n;
         a.out = p->dx;
+        a.stream_out = stream_results(m, k, false);
         a.out_vec = k % 8 == 0 && al16(p->dx);
         const bool vec = dz_vec && rows16(p->weight, p->weight_stride, k, 2);
         launch_product<FWA2_LIN_DT, true, false, FWA2_ACT_NONE>(a, plan(m, k, n, false, 2, cus, vec), vec, st);
