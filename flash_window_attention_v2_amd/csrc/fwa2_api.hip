@@ -440,7 +440,8 @@ static int validate_norm(const fwa2_norm* p, int backward) {
     if (p->kind != FWA2_NORM_LAYER && p->kind != FWA2_NORM_RMS) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: kind %d unknown", p->kind);
     const bool pre = p->placement == FWA2_NORM_PRE;
     if (!pre && p->placement != FWA2_NORM_POST) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: placement %d unknown", p->placement);
-    if (!(p->eps > 0.f && p->eps < INFINITY)) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: eps must be positive");
+    // (not subnormal: 1 / sqrt(var + eps) of a constant row is taken from it alone)
+    if (!(p->eps >= 0x1p-126f && p->eps < INFINITY)) return fail(FWA2_ERR_INVALID_ARGUMENT, "norm: eps must be positive");
     if ((rc = check_norm_sizes(p))) return rc;
     const size_t xb = p->dtype == FWA2_F32 ? 4 : 2, sb = p->stream_dtype == FWA2_F32 ? 4 : 2, wb = p->param_dtype == FWA2_F32 ? 4 : 2;
     const size_t yb = pre ? xb : sb;

@@ -537,25 +537,27 @@ __global__ void __launch_bounds__(norm_block(LPR)) quantize_rows_kernel(const XT
     __shared__ uint32_t red[32];
     int slot = 0;
     const int l = threadIdx.x % LPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
-    const bool ok = row < rows;
-    const int64_t rr = ok ? row : rows - 1;
-    float v[CPL][8];
-    uint32_t amax = 0;
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += (int64_t)gridDim.x * RPB) {
+        const int64_t row = base + threadIdx.x / LPR;
+        const bool ok = row < rows;
+        const int64_t rr = ok ? row : rows - 1;
+        float v[CPL][8];
+        uint32_t amax = 0;
 #pragma unroll
-    for (int c = 0; c < CPL; c++) {
-        const typename Vec8<XT>::V r = row_load8<VEC>(x + rr * xs, 8 * (c * LPR + l), dim);
+        for (int c = 0; c < CPL; c++) {
+            const typename Vec8<XT>::V r = row_load8<VEC>(x + rr * xs, 8 * (c * LPR + l), dim);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            v[c][j] = (float)r[j];
-            amax = MaxU::of(amax, abs_bits(v[c][j]));
+            for (int j = 0; j < 8; j++) {
+                v[c][j] = (float)r[j];
+                amax = MaxU::of(amax, abs_bits(v[c][j]));
+            }
         }
-    }
-    const RowScale sc = scale_of(row_reduce<MaxU, LPR>(amax, red, slot));
-    if (!ok) return;
-    if (l == 0) scale[rr] = sc.scale;
+        const RowScale sc = scale_of(row_reduce<MaxU, LPR>(amax, red, slot));
+        if (!ok) continue;
+        if (l == 0) scale[rr] = sc.scale;
 #pragma unroll
-    for (int c = 0; c < CPL; c++) store_e4m3<VEC>(q + rr * dim, 8 * (c * LPR + l), dim, v[c], sc);
+        for (int c = 0; c < CPL; c++) store_e4m3<VEC>(q + rr * dim, 8 * (c * LPR + l), dim, v[c], sc);
+    }
 }
 
 // ---- launch ---------------------------------------------------------------------------------------------------
@@ -603,11 +605,14 @@ static void backward_typed(const NormArgs& a, bool vec, int blocks, hipStream_t 
     FWA2_NORM_SHAPES(FWA2_GO)
 #undef FWA2_GO
 }
+// A launch has fewer than 2^32 threads: beyond so many workgroups each takes several stretches of rows.
+constexpr int64_t kQuantizeBlocks = 1 << 16;
 template <class XT>
 static void quantize_typed(const void* x, int64_t rows, int dim, int64_t xs, void* q, float* scale, bool vec, hipStream_t st) {
 #define FWA2_GO(LPR, CPL) {                                                                                        \
         constexpr int rpb = norm_block(LPR) / LPR;                                                                  \
-        const dim3 grid((unsigned)((rows + rpb - 1) / rpb)), block(norm_block(LPR));                                \
+        const int64_t tiles = (rows + rpb - 1) / rpb;                                                               \
+        const dim3 grid((unsigned)(tiles < kQuantizeBlocks ? tiles : kQuantizeBlocks)), block(norm_block(LPR));     \
         if (vec) hipLaunchKernelGGL((quantize_rows_kernel<XT, LPR, CPL, true>), grid, block, 0, st,                \
                                     reinterpret_cast<const XT*>(x), rows, dim, xs, reinterpret_cast<uint8_t*>(q), scale); \
         else hipLaunchKernelGGL((quantize_rows_kernel<XT, LPR, CPL, false>), grid, block, 0, st,                   \

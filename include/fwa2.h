@@ -53,7 +53,7 @@ typedef enum fwa2_status {
 typedef enum fwa2_dtype {
     FWA2_F16 = 0,
     FWA2_BF16 = 1,
-    FWA2_F32 = 2 /* only valid as mask_dtype (attn_kernel_forward.py:287) */
+    FWA2_F32 = 2 /* as mask_dtype (attn_kernel_forward.py:287), and for the normalisation further down */
 } fwa2_dtype;
 
 typedef enum fwa2_scale_kind {
@@ -332,7 +332,7 @@ typedef struct fwa2_norm {
     int32_t param_dtype;
     int32_t kind;           /* fwa2_norm_kind */
     int32_t placement;      /* fwa2_norm_place */
-    float   eps;            /* > 0 */
+    float   eps;            /* at least 2^-126 */
     int64_t rows;           /* 1 .. 2^31 - 1 */
     int32_t dim;            /* 1 .. FWA2_NORM_MAX_DIM */
     int32_t gate_dtype;     /* `dtype` or FWA2_F32 */

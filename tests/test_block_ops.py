@@ -62,7 +62,7 @@ def test_norm_validate(lib):
     refuse("dtype or fp32", param_dtype=_abi.E4M3)
     refuse("kind", kind=2)
     refuse("placement", placement=5)
-    for eps in (0.0, -1.0, float("nan"), float("inf")):
+    for eps in (0.0, -1.0, 1e-40, float("nan"), float("inf")):
         refuse("eps", eps=eps)
     refuse("rows", rows=0)
     refuse("rows", rows=1 << 31)

@@ -211,6 +211,14 @@ def test_quantize_rows(dtype, rows, dim):
     assert float(scale[0]) == 1.0 and torch.equal(q.float(), table)
 
 
+def test_quantize_more_rows_than_workgroups():
+    g = _gen(77)
+    x = _rand(g, 70001, 2056, dtype=BF16)       # one workgroup a row, 65536 at most
+    q, scale = fwa2.quantize_rows_func(x)
+    for rows in (slice(0, 50), slice(65500, 65600), slice(69950, 70001)):
+        check_e4m3(q[rows], scale[rows], x[rows].double(), torch.zeros_like(x[rows]).double(), "x8")
+
+
 # ---- matrix product with an epilogue ---------------------------------------------------------------------------------
 LINEAR_SIZES = [(1, 1, 1), (1, 768, 1000), (3, 17, 5), (2, 8, 8), (64, 64, 64), (65, 72, 136), (130, 96, 384), (127, 588, 333),
                 (300, 8, 520), (1000, 100, 64), (33, 1030, 40), (257, 136, 1000), (16, 4096, 24), (5000, 96, 96)]
@@ -318,6 +326,29 @@ def test_linear_views():
     inside(leaf.grad, want, 3 * sum(p.grad.double().abs() for p in parts) * 2.0 ** -8, "shared")
 
 
+def test_linear_single_row_without_leading_dimensions():
+    x, w, b, r, dy = _linear_case(1, 72, 40, BF16, True, True, 19)
+    y = fwa2.fused_linear_func(x[0], w, b, "gelu", r[0])
+    assert y.shape == (40,) and torch.equal(y, fwa2.fused_linear_func(x, w, b, "gelu", r)[0])
+    leaf = x[0].clone().requires_grad_()
+    fwa2.fused_linear_func(leaf, w, b, "gelu").backward(dy[0])
+    value, off = linear_ref(x, w, b, "gelu", None, dy)["dx"]
+    inside(leaf.grad[None], value, rounded(value, off, BF16), "dx")
+    x8, sx = fwa2.quantize_rows_func(x[0])
+    w8, sw = fwa2.quantize_rows_func(w)
+    assert fwa2.fused_linear_fp8_func(x8, sx, w8, sw).shape == (40,)
+
+
+@pytest.mark.parametrize("m", [1, 15, 16, 17, 33, 48, 49, 64, 65])
+def test_linear_few_rows_agree_with_their_definition(m):
+    # the kernel for few rows and its border to the tiles, with contractions that end inside a product
+    for k, n in [(8, 24), (40, 16), (520, 200), (4104, 72)]:
+        x, w, b, r, dy = _linear_case(m, k, n, F16, True, True, m + k)
+        for act, res in ((None, r), ("gelu", None), ("gelu_tanh", r)):
+            value, off = linear_ref(x, w, b, act, res)["y"]
+            inside(fwa2.fused_linear_func(x, w, b, act, res), value, rounded(value, off, F16), f"{k} {n} {act}")
+
+
 def test_linear_only_some_gradients():
     x, w, b, r, dy = _linear_case(100, 72, 40, BF16, True, True, 9)
     full = [t.clone().requires_grad_() for t in (x, w, b, r)]
@@ -333,6 +364,21 @@ def test_linear_long_contraction_and_many_rows():
     for m, k, n in [(20000, 96, 40), (9999, 136, 200), (4097, 33, 17), (70000, 8, 8)]:
         x, w, b, r, dy = _linear_case(m, k, n, BF16, True, False, m)
         _check_linear(x, w, b, None, r, dy, f"{m} ")
+
+
+@pytest.mark.parametrize("m,k,n", [(16500, 64, 136), (16384, 192, 384), (5000, 512, 192), (8200, 520, 392), (4099, 768, 264),
+                                   (8192, 512, 2048), (4100, 1032, 4104), (100, 2048, 2000), (3000, 384, 1160)])
+def test_linear_tiles_of_every_size(m, k, n):
+    # sizes that the host sends to the 128-, 192- and 256-wide tiles forward and backward, whole and with ragged edges
+    x, w, b, r, dy = _linear_case(m, k, n, BF16, True, True, m + k + n)
+    _check_linear(x, w, b, "gelu", None, dy)
+    _check_linear(x, w, b, None, r, dy)
+    x8, sx = fwa2.quantize_rows_func(x)
+    w8, sw = fwa2.quantize_rows_func(w)
+    rows = torch.arange(0, m, max(1, m // 60), device="cuda")
+    y = fwa2.fused_linear_fp8_func(x8, sx, w8, sw, b, "gelu", r)
+    value, off = linear8_ref(x8[rows], sx[rows], w8, sw, b, "gelu", r[rows])
+    inside(y[rows], value, rounded(value, off, BF16), "8 bits")
 
 
 def test_linear_empty_and_far_rows():
