@@ -9,8 +9,9 @@ CPU path and no fallback.
 
 Tensors of any strides are taken; what the kernels cannot address (an inner stride other than 1, rows that overlap or lie
 2^22 elements apart or more) is copied first.  Leading dimensions are flattened to rows.  Every call works on the current
-stream of the tensors' device and can be captured into a graph; gradients are bit-reproducible and cannot be
-differentiated a second time (that raises).
+stream of the tensors' device and can be captured into a graph (a backward pass, as with any autograd operator: while no
+eager graph of the same leaves is alive, whose nodes belong to another stream); gradients are bit-reproducible and
+cannot be differentiated a second time (that raises).
 """
 import torch
 

@@ -17,6 +17,12 @@
 // dW contracts over the rows of the batch and has few output tiles: the rows are split over workgroups, whose fp32
 // partial tiles are added in a fixed order by a second kernel.  dbias is the same contraction against ones and rides on the
 // matrix pipe of the workgroups with the first column tile.
+//
+// What bounds it, measured on MI355X.  Short contractions: memory.  262144 x 96 -> 384 with GELU 66 us for 252 MB
+// (3.8 TB/s; a large copy reaches 5.2, and the stores queue behind a tile's loads); 65536 x 768 -> 192 with a residual 33 us
+// (4.6 TB/s).  Long ones: the matrix pipe.  8192 x 4096 -> 4096 bf16 242 us = 1 137 TFLOP/s (the library's plain product of
+// that size 212 us), 8-bit 129 us = 2 130 TFLOP/s.  Between the two every product of a training step sits near both limits:
+// 16384 x 384 -> 1536, forward with z 38 us (2.9 TB/s), dx 28 us, dW 31 + 10 us.
 #include <initializer_list>
 #include <type_traits>
 
@@ -65,7 +71,8 @@ template <> struct LinElem<FWA2_E4M3> { static constexpr int bytes = 1; };
 // minimax fit over [0, 6], weighted by (u + 0.35) Q(u), value at 0 fixed) gives Q to 8e-7 absolutely and 5e-5 relatively
 // over the fit, and falls on beyond it (6e-16 at 8, 0 from 20 on, where u is cut so that infinity meets a zero).  Eight
 // instructions and one exponential: the library's erff takes about 40, which in the epilogue of a product with few
-// contraction elements (96 -> 384) was more than everything else together (249 us of which 130 by count, 49 by memory).
+// contraction elements (262144 x 96 -> 384) are 130 us of vector instructions next to 49 us of memory traffic; the whole
+// call now takes 66.
 __device__ __forceinline__ float normal_tail(float u) {
     float p = -1.1775869097618852e-06f;
     p = __builtin_fmaf(p, u, 4.9426900659454986e-05f);
@@ -774,11 +781,10 @@ __global__ void __launch_bounds__(64 * WP * WQ, WAVES) linear_kernel(const LinAr
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
-// Up to 64 rows (single tokens, a pooled image): the call reads the weights once and is over; what counts is how soon every
-// load is on its way.  A workgroup owns 16 output columns and its wavefronts split the contraction; operands go from memory
+// Single tokens, a pooled image: the call reads the weights once and is over; what counts is how soon every load is on its
+// way.  A workgroup owns 16 output columns of 16 MQ rows and its wavefronts split the contraction; operands go from memory
 // straight into the registers of 16-row products (no staging, no barrier until the end), partial sums meet in LDS and are
-// added in a fixed order.  1 x 768 -> 1000: 9.0 us on 64 x 64 tiles (24 stages one after the other), see the table at
-// plan_product for the rest.
+// added in a fixed order.  Its limit is that every workgroup gathers its rows of x anew (takes_rows has the figures).
 template <int DT> struct Frag16 {           // v_mfma_f32_16x16x32
     typedef typename Elem<DT>::V8 V;
     static constexpr int BYTES = 64;        // of a row per product
@@ -805,7 +811,7 @@ template <> struct Frag16<FWA2_E4M3> {      // v_mfma_f32_16x16x128
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
     }
 };
-constexpr int kRowsMax = 64, kRowsWaves = 16;
+constexpr int kRowsWaves = 8;
 
 template <int DT, int MQ>       // MQ: groups of 16 rows
 __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinArgs a) {
@@ -814,11 +820,11 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
     __shared__ float sums[kRowsWaves][MQ][16][17];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int l16 = lane & 15, g = lane >> 4;
-    const int p0 = blockIdx.x * 16;
+    const int p0 = blockIdx.x * 16, q0 = blockIdx.y * (16 * MQ);
     const char* prow = a.p + (int64_t)min(p0 + l16, a.np - 1) * a.p_stride;
     const char* qrow[MQ];
 #pragma unroll
-    for (int i = 0; i < MQ; i++) qrow[i] = a.q + (int64_t)min(16 * i + l16, (int)a.nq - 1) * a.q_stride;
+    for (int i = 0; i < MQ; i++) qrow[i] = a.q + (int64_t)min(q0 + 16 * i + l16, (int)a.nq - 1) * a.q_stride;
     f32x4 acc[MQ];
 #pragma unroll
     for (int i = 0; i < MQ; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -832,7 +838,7 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
     if (DT == FWA2_E4M3) p_scale = a.p_scale[p];
 #pragma unroll
     for (int k = 0; k < MQ; k++) {
-        const int q = min((int)(threadIdx.x + k * blockDim.x) >> 4, (int)a.nq - 1);
+        const int q = min(q0 + ((int)(threadIdx.x + k * blockDim.x) >> 4), (int)a.nq - 1);
         res[k] = {};
         q_scale[k] = 1.f;
         if (a.residual != nullptr) res[k] = reinterpret_cast<const RT*>(a.residual + q * a.residual_stride)[p];
@@ -865,14 +871,14 @@ __global__ void __launch_bounds__(64 * kRowsWaves) linear_rows_kernel(const LinA
 #pragma unroll
         for (int k = 0; k < MQ; k++) {
             const int t = threadIdx.x + k * blockDim.x, q = t >> 4;
-            if (t >= MQ * 256 || q >= a.nq || p0 + (t & 15) >= a.np) continue;
+            if (t >= MQ * 256 || q0 + q >= a.nq || p0 + (t & 15) >= a.np) continue;
             float v = 0.f;
             for (int w = 0; w < waves; w++) v += sums[w][q >> 4][q & 15][t & 15];
             const float b = (float)__builtin_bit_cast(OT, bias);
             if constexpr (DT == FWA2_E4M3) v = v * (q_scale[k] * p_scale) + b;
             else v += b;
             asm("" : "+v"(v));
-            const int64_t at = (int64_t)q * a.np + p;
+            const int64_t at = (int64_t)(q0 + q) * a.np + p;
             if (a.z != nullptr) reinterpret_cast<OT*>(a.z)[at] = (OT)v;
             v = act_of(v, a.act);
             asm("" : "+v"(v));
@@ -947,7 +953,7 @@ __global__ void __launch_bounds__(64 * W) linear_sum_kernel(const float* part, i
 
 // dz = dy act'(z), contiguous, and the column sums of dz before its rounding (part_db, one partial row per blockIdx.y).
 // A workgroup owns up to 512 columns (8 per lane, `lanes` lanes a row, a power of two) and a stretch of rows; bound by its
-// three streams.
+// three streams (16384 x 1536: 30 us, 5.0 TB/s).
 constexpr int kActRows = 256;      // at most so many stretches of rows: their partial sums stay small
 template <class E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t dy_stride, const E* z, E* dz, int64_t rows,
@@ -1043,7 +1049,7 @@ struct TileShape {
     int bp, bq, kb, per_cu;     // columns, rows, bytes of the contraction per stage, resident workgroups of a CU
 };
 static constexpr TileShape kTiles[] = {
-    {64, 64, 64, 4},      // T64:    too few output tiles of any other size to fill the chip
+    {64, 64, 128, 3},     // T64:    too few output tiles of any other size to fill the chip; 3 stages, few waits per contraction
     {128, 128, 64, 4},    // T128S:  short contractions: loads and stores bound the call, many workgroups hide each other's
     {128, 128, 128, 2},   // T128
     {192, 128, 128, 2},   // T192P:  column counts that waste less of 192 than of 128 (and equal ones: fewer operand reads)
@@ -1058,13 +1064,17 @@ struct LinPlan {
     int tiles_p;
 };
 
-// The rule, with what it was measured on (MI355X, us, bf16; rows x contraction -> columns):
+// The rule, with what it was measured on (MI355X, us, bf16, operands not in the caches; rows x contraction -> columns):
 //   262144 x   96 ->  384 gelu       T128S  62, T128  94, T192P 106, T256 115, T64  94
 //    65536 x  192 ->  768 gelu, z    T128S  47, T128  50, T192P  54, T256  54, T64  70
 //    16384 x  384 -> 1536 gelu, z    T128S  40, T128  38, T192P  39, T256  44, T64  55
 //    65536 x  768 ->  192 residual   T128S  39, T128  33, T192P  26, T256  32, T64  57
-//     4096 x  768 -> 1536 gelu, z    T128S  23, T128  20, T192P  20, T256  30, T64  29
-//     2048 x 1024 -> 1024 gelu       T128S  16, T128  15, T192P  19, T256  31, T64  14
+//     4096 x  768 -> 1536 gelu, z    T128S  28, T128  25, T192P  24,           T64  27
+//     4096 x 1536 ->  768 residual   T128S  28, T128  21, T192P  25,           T64  22     (T192P: half the CUs)
+//    16384 x  384 ->  384            T128S  13, T128  11, T192P  11,           T64  14
+//    16384 x  384 ->   96 residual   T128S   9, T128   8, T192P  10,           T64   7
+//     2048 x 1024 -> 1024            T128S  15, T128  14,                      T64  11
+//      512 x 4096 -> 1024            T128S  45, T128  43,                      T64  25
 //     8192 x 4096 -> 4096 residual   T128S 375, T128 291, T192P 283, T256 228, T64 665
 // weight gradients (rows of dW x rows of the batch -> columns of dW), splits chosen as below:
 //      384 x 262144 ->  96           T128  49, T192Q 39, T192P 64, T192 50, T256  65
@@ -1088,7 +1098,7 @@ static LinPlan plan_product(int64_t nq, int np, int64_t nk, bool split, int elem
     } else if (nk * elem_bytes <= 384) {
         pl.tile = T128S;
     } else {
-        pl.tile = wide(np) && np > 128 ? T192P : T128;
+        pl.tile = wide(np) && np > 128 && count(T192P) >= cus ? T192P : T128;
     }
     const TileShape& sh = kTiles[pl.tile];
     const int ke = sh.kb / elem_bytes;
@@ -1126,7 +1136,7 @@ static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t s
         return;
     }
     switch (pl.tile) {
-        case T64: FWA2_GO(64, 64, 2, 2, 64, 4, 4); break;
+        case T64: FWA2_GO(64, 64, 2, 2, 128, 3, 3); break;
         case T128S:
             if constexpr (!TURNED) FWA2_GO(128, 128, 2, 2, 64, 2, 3);
             break;
@@ -1143,23 +1153,32 @@ static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t s
 #undef FWA2_GO
 }
 
-// Up to 64 rows take the kernel made for them, whatever the other sizes.
+// Which products linear_rows_kernel takes: up to 16 rows, and any number whose workgroups find a CU each; beyond that the
+// gathering of x costs more than the 64 x 64 tiles' stages, one after the other, do.  Measured (bf16, us, tiles / this
+// kernel, cold weights):
+//     1 x  768 ->  1536   8.2 / 4.5      64 x  768 -> 1536   6.8 /  4.9      256 x 1536 ->  384  10.8 /  6.9
+//     1 x 4096 ->  4096  28.1 / 8.7      64 x 4096 -> 1024  23.9 / 10.3      128 x 4096 -> 1024  24.2 / 13.4
+//     1 x 1024 -> 16384  10.3 / 8.3      16 x 1024 -> 16384 10.8 / 11.1       16 x  384 -> 8192   4.6 /  4.3
+// and beyond the rule:                   32 x 1024 -> 16384 11.2 / 16.0      256 x  768 -> 1536   6.9 /  9.5
+//                                        64 x 4096 ->  4096 28.6 / 25.5      128 x 4096 -> 4096  28.9 / 46.6
+static bool takes_rows(int64_t nq, int np, int cus) {
+    return nq <= 16 || ((nq + 31) / 32) * (int64_t)((np + 15) / 16) <= cus;
+}
+// 16 rows to a workgroup while there is a CU for each, 32 otherwise (64 x 4096 -> 1024: 10.2 / 13.3 us; -> 4096: 32.6 / 25.6);
+// 8 wavefronts, 4 where there are many workgroups (1 x 1024 -> 16384: 8.2 us with 4, 9.8 with 8, 14.1 with 16).
 template <int DT>
-static void launch_rows(const LinArgs& a, hipStream_t st) {
-    const int64_t steps = (a.nk * LinElem<DT>::bytes + Frag16<DT>::BYTES - 1) / Frag16<DT>::BYTES;
-    int waves = kRowsWaves;
-    while (waves > 4 && waves > steps) waves /= 2;
-    const dim3 grid((a.np + 15) / 16), block(64 * waves);
-    if (a.nq <= 16) hipLaunchKernelGGL((linear_rows_kernel<DT, 1>), grid, block, 0, st, a);
-    else if (a.nq <= 32) hipLaunchKernelGGL((linear_rows_kernel<DT, 2>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((linear_rows_kernel<DT, 4>), grid, block, 0, st, a);
+static void launch_rows(const LinArgs& a, int cus, hipStream_t st) {
+    const int64_t columns = (a.np + 15) / 16, groups = (a.nq + 15) / 16;
+    const dim3 block(64 * (columns > 2 * cus ? 4 : kRowsWaves));
+    if (a.nq <= 16 || columns * groups <= cus) hipLaunchKernelGGL((linear_rows_kernel<DT, 1>), dim3(columns, groups), block, 0, st, a);
+    else hipLaunchKernelGGL((linear_rows_kernel<DT, 2>), dim3(columns, (groups + 1) / 2), block, 0, st, a);
 }
 
 // The activations a product is compiled for; the others are decided at run time, row by row of the epilogue.
 template <int DT>
-static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, hipStream_t st) {
-    if (vec && a.nq <= kRowsMax) {
-        launch_rows<DT>(a, st);
+static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, int cus, hipStream_t st) {
+    if (vec && takes_rows(a.nq, a.np, cus)) {
+        launch_rows<DT>(a, cus, st);
         return;
     }
     if (a.act == FWA2_ACT_NONE) launch_product<DT, false, false, FWA2_ACT_NONE>(a, pl, vec, st);
@@ -1168,7 +1187,8 @@ static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, hipStr
 }
 
 // Tiles for operands that go through registers: 128 wide when those fill the chip twice (their loads are waited for stage by
-// stage, so there have to be several workgroups to a CU), 64 otherwise.
+// stage, so there have to be several workgroups to a CU), 64 otherwise.  Measured (us, 64 / 128 wide): 1225 x 588 -> 333
+// 10.6 / 17.7 and its weight gradient 10.9 / 13.2; 4099 x 585 -> 1161 25.9 / 23.8, 40.9 / 50.6; 16389 x 585 -> 1161 97 / 63.
 static LinPlan plan_unaligned(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
     LinPlan pl;
     auto count = [&](int b) { return ((nq + b - 1) / b) * ((np + b - 1) / b); };
@@ -1220,7 +1240,7 @@ static LinArgs forward_args(const fwa2_linear* p) {
 #if FWA2_HALF == 3
 void linear_forward_e4m3(const fwa2_linear* p, int cus, hipStream_t st) {
     const bool vec = rows16(p->x, p->x_stride, p->in_features, 1) && rows16(p->weight, p->weight_stride, p->in_features, 1);
-    launch_forward<FWA2_E4M3>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 1, cus, vec), vec, st);
+    launch_forward<FWA2_E4M3>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 1, cus, vec), vec, cus, st);
 }
 #else
 #if FWA2_HALF == 1
@@ -1232,7 +1252,7 @@ void linear_forward_e4m3(const fwa2_linear* p, int cus, hipStream_t st) {
 #endif
 void FWA2_LIN_FN(linear_forward)(const fwa2_linear* p, int cus, hipStream_t st) {
     const bool vec = rows16(p->x, p->x_stride, p->in_features, 2) && rows16(p->weight, p->weight_stride, p->in_features, 2);
-    launch_forward<FWA2_LIN_DT>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 2, cus, vec), vec, st);
+    launch_forward<FWA2_LIN_DT>(forward_args(p), plan(p->rows, p->out_features, p->in_features, false, 2, cus, vec), vec, cus, st);
 }
 static size_t dz_bytes(int64_t m, int n) { return ((size_t)m * n * 2 + 255) / 256 * 256; }
 static size_t act_bytes(const fwa2_linear* p, int cus) {

@@ -366,6 +366,14 @@ def test_linear_long_contraction_and_many_rows():
         _check_linear(x, w, b, None, r, dy, f"{m} ")
 
 
+@pytest.mark.parametrize("m,k,n", [(31, 4096, 1000), (97, 520, 96), (255, 1536, 384), (300, 264, 40), (1, 1024, 16384), (16, 72, 8200)])
+def test_linear_few_workgroups_agree_with_their_definition(m, k, n):
+    """Groups of 16 and of 32 rows and 4 wavefronts to a workgroup, with products that end inside each."""
+    x, w, b, r, dy = _linear_case(m, k, n, BF16, True, True, m + k)
+    value, off = linear_ref(x, w, b, "gelu", r)["y"]
+    inside(fwa2.fused_linear_func(x, w, b, "gelu", r), value, rounded(value, off, BF16), "y")
+
+
 @pytest.mark.parametrize("m,k,n", [(16500, 64, 136), (16384, 192, 384), (5000, 512, 192), (8200, 520, 392), (4099, 768, 264),
                                    (8192, 512, 2048), (4100, 1032, 4104), (100, 2048, 2000), (3000, 384, 1160)])
 def test_linear_tiles_of_every_size(m, k, n):
