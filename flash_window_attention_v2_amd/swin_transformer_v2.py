@@ -67,8 +67,8 @@ def _hooked(*modules):
 class Mlp(nn.Module):
     """fc1, activation, fc2.  With `is_fused` the products run on the library's kernels (the activation in the epilogue of
     the first) wherever those apply: on the GPU in half precision, without active dropout, with an activation the library
-    knows.  With `fp8` both products of a call that records no gradient take 8-bit rows: weights quantised once per
-    version, activations row by row."""
+    knows.  With `fp8` both products of a call that records no gradient take 8-bit rows: activations and, unless
+    `hold_weights8` keeps them, weights quantised row by row."""
 
     is_fused = False
     fp8 = False
@@ -111,19 +111,26 @@ class Mlp(nn.Module):
             return False
         return not (torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())))
 
-    def weights8(self):
-        """((fc1 weight, scale), (fc2 weight, scale)) in 8 bits, kept until a weight changes (tensors that track no
-        modifications, as those made under torch.inference_mode, are quantised on every call)."""
-        ws = (self.fc1.weight, self.fc2.weight)
-        key = tuple((tensor_version(w), w.data_ptr(), w.dtype, w.device) for w in ws)
-        held = self._weights8
-        if held is not None and held[0] == key and all(k[0] is not None for k in key):
-            return held[1]
+    def _weights_key(self):
+        return tuple((tensor_version(w), w.data_ptr(), w.dtype, w.device) for w in (self.fc1.weight, self.fc2.weight))
+
+    def _quantize_weights(self):
         with torch.no_grad():
-            made = tuple(quantize_rows_func(w) for w in ws)
-        if not torch.cuda.is_current_stream_capturing():
-            self._weights8 = (key, made)
-        return made
+            return tuple(quantize_rows_func(w) for w in (self.fc1.weight, self.fc2.weight))
+
+    def hold_weights8(self, hold=True):
+        """Quantise the weights now and keep them for the calls that follow (or, with hold=False, let them go): for weights
+        that no longer change.  After an edit in place that torch records they are quantised on every call again; after one
+        that it does not record (through `.data`, by replaying a captured graph) call this once more."""
+        key = self._weights_key()
+        keep = hold and self.fp8 and all(k[0] is not None for k in key)
+        self._weights8 = (key, self._quantize_weights()) if keep else None
+
+    def weights8(self):
+        """((fc1 weight, scale), (fc2 weight, scale)) in 8 bits: the held ones, or made for this call."""
+        if self._weights8 is not None and self._weights8[0] == self._weights_key():
+            return self._weights8[1]
+        return self._quantize_weights()
 
     def forward_fp8(self, x8, scale, dtype):
         """The MLP over 8-bit rows (`residual_norm_fp8_func` or `quantize_rows_func` made them), result in `dtype`."""
@@ -575,7 +582,8 @@ class SwinTransformerV2(nn.Module):
     """Hierarchical Swin V2 classifier with the reference's constructor arguments and parameter
     names (swin_transformer_v2.py:668-822).  Two arguments go beyond it: `is_fused` runs the MLPs and the residual
     post-normalisations of the blocks on the library's kernels (fewer roundings, so results differ in the last bits; off by
-    default), `fp8_mlp` with it the MLPs of calls that record no gradient on 8-bit rows."""
+    default), `fp8_mlp` with it the MLPs of calls that record no gradient on 8-bit rows (`hold_weights8`
+    keeps their weights)."""
 
     def __init__(self, img_size=256, patch_size=4, in_chans=3, num_classes=1000, embed_dim=96, depths=[2, 2, 6, 2],
                  num_heads=[3, 6, 12, 24], window_size=8, is_flash=True, mlp_ratio=4., qkv_bias=True, drop_rate=0.,
@@ -629,6 +637,12 @@ class SwinTransformerV2(nn.Module):
         elif isinstance(m, nn.LayerNorm):
             nn.init.zeros_(m.bias)
             nn.init.ones_(m.weight)
+
+    def hold_weights8(self, hold=True):
+        """`Mlp.hold_weights8` of every block: the 8-bit weights of a model that is only evaluated from here on."""
+        for m in self.modules():
+            if isinstance(m, Mlp):
+                m.hold_weights8(hold)
 
     @torch.jit.ignore
     def no_weight_decay(self):

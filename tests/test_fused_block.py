@@ -131,13 +131,19 @@ def test_fp8_mlp(monkeypatch):
     assert len(calls) == 8
     # operands of 2^-4 half steps in the MLPs of four blocks whose outputs are normalised and added to a stream
     assert float((y.float() - want.float()).norm() / want.float().norm()) <= 2.0 ** -3
-    held = fp8.layers[0].blocks[0].mlp._weights8
+    mlp = fp8.layers[0].blocks[0].mlp
     with torch.no_grad():
-        fp8(x)
-        assert fp8.layers[0].blocks[0].mlp._weights8 is held
-        fp8.layers[0].blocks[0].mlp.fc1.weight.mul_(2)      # edited in place: quantised again
-        fp8(x)
-        assert fp8.layers[0].blocks[0].mlp._weights8 is not held
+        first = fp8(x)
+        fp8.hold_weights8()                 # the same weights, quantised once
+        held = mlp.weights8()
+        assert mlp.weights8() is held and torch.equal(fp8(x), first)
+        mlp.fc1.weight.mul_(2)              # an edit that is recorded: no longer those
+        assert mlp.weights8() is not held and torch.equal(mlp.weights8()[0][1], held[0][1] * 2)
+        assert not torch.equal(fp8(x), first)
+        fp8.hold_weights8(False)
+        second = fp8(x)
+        mlp.fc1.weight.data.mul_(0.5)       # one that is not: nothing is kept between calls
+        assert torch.equal(fp8(x), first) and not torch.equal(second, first)
     calls.clear()
     fp8(x).sum().backward()                                  # with gradients the products stay in 16 bits
     assert not calls and fp8.layers[0].blocks[0].mlp.fc1.weight.grad is not None
