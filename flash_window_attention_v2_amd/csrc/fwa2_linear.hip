@@ -1044,7 +1044,7 @@ static ActPlan plan_act(int64_t rows, int n, int cus) {
 
 // ---- launch ---------------------------------------------------------------------------------------------------
 // The tile a product runs on, and how its contraction is split.
-enum Tile { T64, T128S, T128, T192P, T192Q, T192, T256 };
+enum Tile { T64, T128S, T128, T192P, T192Q, T192, T256, T256P };
 struct TileShape {
     int bp, bq, kb, per_cu;     // columns, rows, bytes of the contraction per stage, resident workgroups of a CU
 };
@@ -1056,6 +1056,7 @@ static constexpr TileShape kTiles[] = {
     {128, 192, 128, 2},   // T192Q:  the same for the rows; weight gradients only, as is
     {192, 192, 128, 1},   // T192:   both
     {256, 256, 128, 1},   // T256:   large products, 8 wavefronts: LDS reads per product fall with the tile's edge
+    {256, 128, 64, 2},    // T256P:  contractions not quite as short: half as many tiles' first loads to wait for
 };
 struct LinPlan {
     Tile tile;
@@ -1066,7 +1067,8 @@ struct LinPlan {
 
 // The rule, with what it was measured on (MI355X, us, bf16, operands not in the caches; rows x contraction -> columns):
 //   262144 x   96 ->  384 gelu       T128S  62, T128  94, T192P 106, T256 115, T64  94
-//    65536 x  192 ->  768 gelu, z    T128S  47, T128  50, T192P  54, T256  54, T64  70
+//    65536 x  192 ->  768 gelu, z    T128S  62, T128  67, T192P  65, T256P  58
+//    65536 x  192 ->  768 (dx)       T128S  49, T128  49, T192P  44, T256P  38
 //    16384 x  384 -> 1536 gelu, z    T128S  40, T128  38, T192P  39, T256  44, T64  55
 //    65536 x  768 ->  192 residual   T128S  39, T128  33, T192P  26, T256  32, T64  57
 //     4096 x  768 -> 1536 gelu, z    T128S  28, T128  25, T192P  24,           T64  27
@@ -1096,7 +1098,8 @@ static LinPlan plan_product(int64_t nq, int np, int64_t nk, bool split, int elem
     } else if (small || count(T128) * 10 < 6 * cus) {
         pl.tile = T64;
     } else if (nk * elem_bytes <= 384) {
-        pl.tile = T128S;
+        const bool whole = up(np, 256) * 2 <= up(np, 128) && count(T256P) >= 2 * cus;
+        pl.tile = nk * elem_bytes > 192 && whole ? T256P : T128S;
     } else {
         pl.tile = wide(np) && np > 128 && count(T192P) >= cus ? T192P : T128;
     }
@@ -1149,6 +1152,9 @@ static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t s
             if constexpr (TURNED) FWA2_GO(192, 192, 2, 2, 128, 2, 1);
             break;
         case T256: FWA2_GO(256, 256, 2, 4, 128, 2, 2); break;
+        case T256P:
+            if constexpr (!TURNED) FWA2_GO(256, 128, 2, 2, 64, 2, 2);
+            break;
     }
 #undef FWA2_GO
 }

@@ -366,6 +366,23 @@ def test_linear_long_contraction_and_many_rows():
         _check_linear(x, w, b, None, r, dy, f"{m} ")
 
 
+@pytest.mark.parametrize("m,k,n", [(22000, 128, 1000), (66000, 192, 248), (65541, 104, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_wide_tiles_of_short_contractions(m, k, n, dtype):
+    """256 columns to a tile, tiles that end inside, forward and (contraction n) backward; sampled rows."""
+    x, w, b, r, dy = _linear_case(m, k, n, dtype, True, True, m)
+    y = fwa2.fused_linear_func(x, w, b, "gelu", r)
+    rows = torch.cat([torch.arange(0, m, 997), torch.arange(m - 140, m)]).to(x.device)
+    value, off = linear_ref(x[rows], w, b, "gelu", r[rows])["y"]
+    inside(y[rows], value, rounded(value, off, dtype), "y")
+    leaf = dy.clone().requires_grad_()          # dy W, whose contraction is n: through the product of W transposed
+    wt = w.t().contiguous()
+    out = fwa2.fused_linear_func(leaf, wt)
+    back, = torch.autograd.grad(out, [leaf], x)
+    value, off = linear_ref(dy[rows], wt, None, None, None, x[rows])["dx"]
+    inside(back[rows], value, rounded(value, off, dtype), "dx")
+
+
 @pytest.mark.parametrize("m,k,n", [(31, 4096, 1000), (97, 520, 96), (255, 1536, 384), (300, 264, 40), (1, 1024, 16384), (16, 72, 8200)])
 def test_linear_few_workgroups_agree_with_their_definition(m, k, n):
     """Groups of 16 and of 32 rows and 4 wavefronts to a workgroup, with products that end inside each."""
