@@ -443,7 +443,9 @@ class SwinTransformerBlock(nn.Module):
         n = self.norm1
         recorded = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
                                                    (shortcut, getattr(n, "weight", None), getattr(n, "bias", None)))
-        if not recorded and self.mlp.fp8_ready(x) and self._norm_fused(n, x, shortcut) and not _hooked(self.mlp):
+        # any module may stand in the Mlp's place, and what is gone around below is the Mlp's own forward
+        if (not recorded and type(self.mlp) is Mlp and self.mlp.fp8_ready(x) and self._norm_fused(n, x, shortcut)
+                and not _hooked(self.mlp)):
             # the rows leave the first norm in 8 bits next to the stream
             dtype = self.mlp.fused_dtype(x)
             with torch.no_grad():

@@ -1,0 +1,54 @@
+"""Where the block's second half leaves its modules to themselves: what a user may have put into a block, or hung on its parts,
+has to happen with `is_fused` as without it."""
+import pytest
+import torch
+import torch.nn as nn
+
+from flash_window_attention_v2_amd import swin_transformer_v2 as swin
+
+
+def _block(**kw):
+    torch.manual_seed(0)
+    blk = swin.SwinTransformerBlock(**{**dict(dim=16, input_resolution=(8, 8), num_heads=1, window_size=4, is_flash=False), **kw})
+    for n in (blk.norm1, blk.norm2):
+        nn.init.normal_(n.weight, 1.0, 0.1)
+    return blk
+
+
+@pytest.mark.parametrize("is_fused", [False, True])
+@pytest.mark.parametrize("grad", [torch.no_grad, torch.inference_mode, torch.enable_grad])
+def test_a_block_takes_any_module_as_its_mlp(is_fused, grad):
+    blk = _block(is_fused=is_fused, fp8_mlp=is_fused).eval()
+    x = torch.randn(2, 64, 16)
+    for mlp in (nn.Sequential(nn.Linear(16, 16), nn.GELU()), nn.Identity()):
+        blk.mlp = mlp
+        with grad():
+            s = x + blk.norm1(_attention(blk, x))
+            assert torch.allclose(blk(x), s + blk.norm2(mlp(s)), atol=1e-6)
+
+
+def _attention(blk, x):
+    """The block's first half, by its modules."""
+    windows = swin.window_partition(x.view(-1, 8, 8, 16), 4).view(-1, 16, 16)
+    return swin.window_reverse(blk.attn(windows).view(-1, 4, 4, 16), 4, 8, 8).reshape(x.shape)
+
+
+def test_an_mlp_of_another_class_is_called(monkeypatch):
+    # the 8-bit path goes around the Mlp's forward: only where that is the one it stands for
+    class Other(swin.Mlp):
+        def forward(self, x):
+            called.append(1)
+            return x
+
+    called = []
+    blk = _block(is_fused=True, fp8_mlp=True).eval()
+    blk.mlp = Other(16, 64)
+    monkeypatch.setattr(swin.Mlp, "fp8_ready", lambda self, x: True)
+    monkeypatch.setattr(swin.Mlp, "fused_dtype", lambda self, x: torch.float16)
+    monkeypatch.setattr(swin.Mlp, "forward_fp8", lambda self, x8, scale, dtype: x8)
+    monkeypatch.setattr(blk, "_norm_fused", lambda *a: True)
+    monkeypatch.setattr(swin, "residual_norm_func", lambda x, s, *a, **k: s + x)
+    monkeypatch.setattr(swin, "residual_norm_fp8_func", lambda x, s, *a, **k: (s + x, s + x, None))
+    with torch.no_grad():
+        blk._second_half(torch.randn(2, 64, 16), torch.randn(2, 64, 16))
+    assert called
