@@ -358,6 +358,8 @@ class SwinTransformerBlock(nn.Module):
     """(Shifted-)window attention + MLP with residual post-normalisation
     (swin_transformer_v2.py:318-447)."""
 
+    is_fused = False
+
     def __init__(self, dim, input_resolution, num_heads, window_size=7, shift_size=0, is_flash=True, mlp_ratio=4.,
                  qkv_bias=True, drop=0., attn_drop=0., drop_path=0., act_layer=nn.GELU, norm_layer=nn.LayerNorm,
                  pretrained_window_size=0, is_fused=False, fp8_mlp=False):

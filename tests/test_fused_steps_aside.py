@@ -52,3 +52,14 @@ def test_an_mlp_of_another_class_is_called(monkeypatch):
     with torch.no_grad():
         blk._second_half(torch.randn(2, 64, 16), torch.randn(2, 64, 16))
     assert called
+
+
+def test_a_block_saved_without_is_fused_still_runs():
+    # a block pickled whole before it had the attribute
+    blk = _block()
+    blk.__dict__.pop("is_fused", None)
+    x = torch.randn(2, 64, 16)
+    want = _block()(x)
+    assert torch.equal(blk(x), want)
+    with torch.no_grad():
+        assert torch.equal(blk(x), want)
