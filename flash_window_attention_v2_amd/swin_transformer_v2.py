@@ -87,11 +87,17 @@ class Mlp(nn.Module):
             return "gelu" if self.act.approximate == "none" else "gelu_tanh"
         return {nn.SiLU: "silu", nn.ReLU: "relu"}.get(type(self.act))
 
+    def _drops(self):
+        """Whether `drop` may change what passes through it; its own mode decides, whatever this module's is."""
+        if type(self.drop) is nn.Dropout:
+            return self.drop.training and self.drop.p > 0
+        return type(self.drop) is not nn.Identity
+
     def fused_dtype(self, x):
         """The dtype the fused products would run in for `x`, or None where they do not apply."""
         if not (self.is_fused and x.is_cuda and self._activation()):
             return None
-        if type(self.fc1) is not nn.Linear or type(self.fc2) is not nn.Linear or (self.training and self.drop.p > 0):
+        if type(self.fc1) is not nn.Linear or type(self.fc2) is not nn.Linear or self._drops():
             return None
         if _hooked(self.fc1, self.act, self.fc2, self.drop):
             return None

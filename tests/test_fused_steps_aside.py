@@ -63,3 +63,32 @@ def test_a_block_saved_without_is_fused_still_runs():
     assert torch.equal(blk(x), want)
     with torch.no_grad():
         assert torch.equal(blk(x), want)
+
+
+class OnGpu:
+    """What the decisions look at of an input."""
+    is_cuda, dtype, requires_grad, shape = True, torch.bfloat16, False, (2, 64, 16)
+
+
+def _mlp(**kw):
+    mlp = swin.Mlp(16, 64, **kw).to(torch.bfloat16)
+    mlp.is_fused = True
+    return mlp
+
+
+def test_dropout_is_judged_by_its_own_mode():
+    mlp = _mlp(drop=0.5)
+    assert mlp.fused_dtype(OnGpu) is None                    # training: active
+    assert mlp.eval().fused_dtype(OnGpu) is torch.bfloat16
+    mlp.drop.train()                                         # Monte-Carlo dropout: a module in evaluation drops all the same
+    assert mlp.fused_dtype(OnGpu) is None
+    mlp.train()
+    mlp.drop.eval()
+    assert mlp.fused_dtype(OnGpu) is torch.bfloat16
+    mlp.drop.train()
+    mlp.drop.p = 0.0
+    assert mlp.fused_dtype(OnGpu) is torch.bfloat16
+    mlp.drop = nn.Identity()                                 # a model without its dropout modules
+    assert mlp.fused_dtype(OnGpu) is torch.bfloat16
+    mlp.drop = nn.AlphaDropout(0.5).eval()
+    assert mlp.fused_dtype(OnGpu) is None
