@@ -433,9 +433,10 @@ class SwinTransformerBlock(nn.Module):
         return not torch.is_autocast_enabled() or shortcut.dtype == torch.float32
 
     def _gate(self, x):
-        """Stochastic depth's factor per sample (0 or 1 / keep), or None; drawn as `drop_path` draws it."""
+        """Stochastic depth's factor per sample (0 or 1 / keep), or None; drawn as `drop_path` draws it, in that module's own
+        mode."""
         p = self.drop_path.drop_prob if isinstance(self.drop_path, DropPath) else 0.
-        if p == 0. or not self.training:
+        if p == 0. or not self.drop_path.training:
             return None
         keep = 1.0 - p
         return x.new_empty((x.shape[0],) + (1,) * (x.dim() - 1)).bernoulli_(keep).float() / keep

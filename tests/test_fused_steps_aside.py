@@ -92,3 +92,17 @@ def test_dropout_is_judged_by_its_own_mode():
     assert mlp.fused_dtype(OnGpu) is torch.bfloat16
     mlp.drop = nn.AlphaDropout(0.5).eval()
     assert mlp.fused_dtype(OnGpu) is None
+
+
+@pytest.mark.parametrize("block_mode", [False, True])
+@pytest.mark.parametrize("path_mode", [False, True])
+def test_stochastic_depth_is_judged_by_its_own_mode(block_mode, path_mode):
+    blk = _block(drop_path=0.4, is_fused=True).train(block_mode)
+    blk.drop_path.train(path_mode)
+    x = torch.randn(64, 64, 16)
+    torch.manual_seed(3)
+    want = blk.drop_path(x)
+    torch.manual_seed(3)
+    gate = blk._gate(x)
+    assert (gate is None) == (not path_mode)
+    assert torch.allclose(want, x if gate is None else gate * x)
