@@ -106,3 +106,25 @@ def test_stochastic_depth_is_judged_by_its_own_mode(block_mode, path_mode):
     gate = blk._gate(x)
     assert (gate is None) == (not path_mode)
     assert torch.allclose(want, x if gate is None else gate * x)
+
+
+def _fits(blk):
+    """Whether the block's two norms and its Mlp would run fused, by what they look at before a call."""
+    x = OnGpu()
+    x.shape = (2, 64, 16)
+    return blk._norm_fused(blk.norm1, x, x), blk.mlp.fused_dtype(x) is not None, blk._norm_fused(blk.norm2, x, x)
+
+
+def _fused_block(**kw):
+    return _block(is_fused=True, **kw).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["forward", "forward_pre", "full_backward", "full_backward_pre"])
+def test_hooks_of_all_modules_are_seen(kind):
+    assert _fits(_fused_block()) == (True, True, True)
+    hook = getattr(torch.nn.modules.module, f"register_module_{kind}_hook")(lambda *a: None)
+    try:
+        assert _fits(_fused_block()) == (False, False, False)
+    finally:
+        hook.remove()
+    assert _fits(_fused_block()) == (True, True, True)
