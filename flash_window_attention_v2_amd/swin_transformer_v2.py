@@ -60,12 +60,14 @@ def shifted_window_attn_mask(resolution, window_size, shift_size):
 
 
 def _hooked(*modules):
-    """Whether any of the modules carries hooks, or all modules do: a call around a module's forward would skip them."""
+    """Whether a call around the forward of any of the modules would skip something that was hung on it: hooks, its own or
+    those of all modules, or a `forward` that replaces the class's on the instance."""
     every = nn.modules.module
     if (every._global_forward_hooks or every._global_forward_pre_hooks or every._global_backward_hooks
             or every._global_backward_pre_hooks):
         return True
-    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules)
+    return any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+               or "forward" in m.__dict__ for m in modules)
 
 
 class Mlp(nn.Module):

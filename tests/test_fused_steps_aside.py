@@ -128,3 +128,32 @@ def test_hooks_of_all_modules_are_seen(kind):
     finally:
         hook.remove()
     assert _fits(_fused_block()) == (True, True, True)
+
+
+def test_a_forward_replaced_on_the_instance_is_seen():
+    def replaced(m):
+        forward = m.forward
+        m.forward = lambda *a: forward(*a)
+
+    for part, want in (("norm1", (False, True, True)), ("norm2", (True, True, False)), ("drop_path", (False, True, False)),
+                       ("mlp.fc1", (True, False, True)), ("mlp.act", (True, False, True)), ("mlp.fc2", (True, False, True)),
+                       ("mlp.drop", (True, False, True))):
+        blk = _fused_block(drop_path=0.1, drop=0.1).eval()
+        assert _fits(blk) == (True, True, True)
+        replaced(blk.get_submodule(part))
+        assert _fits(blk) == want, part
+
+
+def test_a_forward_replaced_on_the_mlp_is_called(monkeypatch):
+    blk = _block(is_fused=True, fp8_mlp=True).eval()
+    called = []
+    blk.mlp.forward = lambda x: (called.append(1), x)[1]
+    monkeypatch.setattr(swin.Mlp, "fp8_ready", lambda self, x: True)
+    monkeypatch.setattr(swin.Mlp, "fused_dtype", lambda self, x: torch.float16)
+    monkeypatch.setattr(swin.Mlp, "forward_fp8", lambda self, x8, scale, dtype: x8)
+    monkeypatch.setattr(blk, "_norm_fused", lambda *a: True)
+    monkeypatch.setattr(swin, "residual_norm_func", lambda x, s, *a, **k: s + x)
+    monkeypatch.setattr(swin, "residual_norm_fp8_func", lambda x, s, *a, **k: (s + x, s + x, None))
+    with torch.no_grad():
+        blk._second_half(torch.randn(2, 64, 16), torch.randn(2, 64, 16))
+    assert called
