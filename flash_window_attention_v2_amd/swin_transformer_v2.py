@@ -433,6 +433,8 @@ class SwinTransformerBlock(nn.Module):
             return False
         if norm.normalized_shape != (x.shape[-1],) or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             return False
+        if not 2.0 ** -126 <= norm.eps <= torch.finfo(torch.float32).max:      # what the kernels take (no subnormal, no zero)
+            return False
         if shortcut.dtype not in (x.dtype, torch.float32) or norm.weight.dtype not in (x.dtype, torch.float32):
             return False
         # under autocast the framework's norm returns fp32, and with it the sum

@@ -157,3 +157,14 @@ def test_a_forward_replaced_on_the_mlp_is_called(monkeypatch):
     with torch.no_grad():
         blk._second_half(torch.randn(2, 64, 16), torch.randn(2, 64, 16))
     assert called
+
+
+def test_an_eps_that_the_kernels_refuse_steps_aside():
+    for eps in (0.0, 1e-40, 1e39):
+        blk = _fused_block()
+        blk.norm1.eps = eps
+        assert _fits(blk) == (False, True, True)
+    for eps in (2.0 ** -126, 1e-12, 3e38):
+        blk = _fused_block()
+        blk.norm2.eps = eps
+        assert _fits(blk) == (True, True, True)
