@@ -132,17 +132,30 @@ class Mlp(nn.Module):
 
     def hold_weights8(self, hold=True):
         """Quantise the weights now and keep them for the calls that follow (or, with hold=False, let them go): for weights
-        that no longer change.  After an edit in place that torch records they are quantised on every call again; after one
-        that it does not record (through `.data`, by replaying a captured graph) call this once more."""
+        that no longer change.  After an edit in place that torch records, or with other parameters in their place, they are
+        quantised on every call again; after an edit that torch does not record (through `.data`, by replaying a captured
+        graph) call this once more."""
+        weights = (self.fc1.weight, self.fc2.weight)
         key = self._weights_key()
         keep = hold and self.fp8 and all(k[0] is not None for k in key)
-        self._weights8 = (key, self._quantize_weights()) if keep else None
+        # The parameters themselves are compared later on, and their memory is kept with the rows made of it: were it freed, a
+        # successor could get the same address and count its edits from the same number.
+        self._weights8 = (key, weights, self._quantize_weights(), [w.detach() for w in weights]) if keep else None
 
     def weights8(self):
         """((fc1 weight, scale), (fc2 weight, scale)) in 8 bits: the held ones, or made for this call."""
-        if self._weights8 is not None and self._weights8[0] == self._weights_key():
-            return self._weights8[1]
+        held = self._weights8
+        if (held is not None and held[0] == self._weights_key() and held[1][0] is self.fc1.weight
+                and held[1][1] is self.fc2.weight):
+            return held[2]
         return self._quantize_weights()
+
+    def _apply(self, fn, *args, **kwargs):
+        # .to() / .half() put other memory under the parameters: the held rows would only keep the old one alive
+        super()._apply(fn, *args, **kwargs)
+        if self._weights8 is not None and self._weights8[0] != self._weights_key():
+            self._weights8 = None
+        return self
 
     def forward_fp8(self, x8, scale, dtype):
         """The MLP over 8-bit rows (`residual_norm_fp8_func` or `quantize_rows_func` made them), result in `dtype`."""

@@ -1,5 +1,7 @@
 """Where the block's second half leaves its modules to themselves: what a user may have put into a block, or hung on its parts,
 has to happen with `is_fused` as without it."""
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
@@ -168,3 +170,85 @@ def test_an_eps_that_the_kernels_refuse_steps_aside():
         blk = _fused_block()
         blk.norm2.eps = eps
         assert _fits(blk) == (True, True, True)
+
+
+# ---- held 8-bit weights ------------------------------------------------------------------------------------------------
+@pytest.fixture
+def holding(monkeypatch):
+    """An Mlp whose 8-bit rows are made on the CPU, by copies that can be told from the weights they were made of."""
+    monkeypatch.setattr(swin, "quantize_rows_func", lambda w: (w.detach().clone(), w.detach().abs().amax(-1)))
+    mlp = swin.Mlp(16, 64)
+    mlp.is_fused = mlp.fp8 = True
+    mlp.hold_weights8()
+    assert mlp.weights8() is mlp.weights8()
+    return mlp
+
+
+def _current(mlp):
+    return all(torch.equal(q, m.weight) for (q, _), m in zip(mlp.weights8(), (mlp.fc1, mlp.fc2)))
+
+
+def test_held_weights_belong_to_their_parameters(holding, monkeypatch):
+    # another parameter of the same size may get the address, and the version counter, of the one that was freed
+    monkeypatch.setattr(swin.Mlp, "_weights_key", lambda self: "the same for both", raising=False)
+    holding.hold_weights8()
+    held = holding.weights8()
+    with torch.no_grad():
+        holding.fc1.weight = nn.Parameter(torch.randn(64, 16))
+    assert holding.weights8() is not held and _current(holding)
+
+
+def test_held_weights_after_replacements(holding):
+    for _ in range(3):
+        holding.hold_weights8()
+        holding.load_state_dict({k: torch.randn_like(v) for k, v in holding.state_dict().items()}, assign=True)
+        assert _current(holding)
+        with torch.no_grad():
+            holding.fc2.weight = nn.Parameter(torch.randn(16, 64))
+        assert _current(holding)
+
+
+def test_the_storage_of_held_weights_is_not_given_away(holding):
+    # .data of one parameter replaced twice: a storage that had been freed in between could come back under its address
+    old = holding.fc1.weight.data_ptr()
+    holding.fc1.weight.data = torch.zeros(64, 16)
+    for _ in range(8):
+        holding.fc1.weight.data = torch.randn(64, 16)
+        assert holding.fc1.weight.data_ptr() != old and _current(holding)
+
+
+def test_conversions_let_held_weights_go(holding):
+    held = holding.weights8()
+    holding.to("cpu")                       # nothing moves
+    assert holding.weights8() is held
+    holding.double()
+    assert holding._weights8 is None and _current(holding)
+
+
+def test_modules_with_held_weights_are_copied_and_saved(holding, tmp_path):
+    twin = copy.deepcopy(holding)
+    assert _current(twin)
+    with torch.no_grad():
+        twin.fc1.weight.mul_(3)
+    assert _current(twin) and _current(holding)
+    torch.save(holding, tmp_path / "mlp.pt")
+    assert _current(torch.load(tmp_path / "mlp.pt", weights_only=False))
+
+
+@pytest.mark.gpu
+def test_held_weights_on_the_gpu_after_replacements():
+    mlp = swin.Mlp(64, 256).cuda().to(torch.bfloat16)
+    mlp.is_fused = mlp.fp8 = True
+    x = torch.randn(5, 64, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        for _ in range(3):
+            mlp.hold_weights8()
+            held = mlp(x)
+            mlp.hold_weights8(False)
+            assert torch.equal(mlp(x), held)
+            mlp.hold_weights8()
+            state = {k: torch.randn_like(v) for k, v in mlp.state_dict().items()}
+            mlp.load_state_dict(state, assign=True)
+            got = mlp(x)
+            mlp.hold_weights8(False)
+            assert torch.equal(mlp(x), got) and not torch.equal(got, held)
