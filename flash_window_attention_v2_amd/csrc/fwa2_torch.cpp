@@ -8,6 +8,7 @@
 // Python functions in block_ops.py that call this.
 #include <torch/extension.h>
 
+#include <ATen/FuncTorchTLS.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -96,6 +97,16 @@ bool wants_grad(std::initializer_list<const Optional*> ts) {
     return false;
 }
 
+// What follows a computation from outside does not see into these functions.  A backward pass is recorded by their nodes; a
+// forward-mode derivative that an input carries would be lost, and so would what the transforms of torch.func keep.
+bool has_forward_grad(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_forward_grad(const Optional& t) { return t.has_value() && has_forward_grad(*t); }
+template <class... T>
+void refuse_unseen(const T&... ts) {
+    if ((has_forward_grad(ts) || ...)) throw StatusError(FWA2_ERR_UNSUPPORTED, "the operator has no forward-mode derivative");
+    if (const auto& transforms = at::functorch::functorchTLSAccessor()) transforms->checkSupportsCppAutogradFunction();
+}
+
 // ---- matrix products ----
 fwa2_linear linear_description(const Rows& x, const Rows& w, int64_t rows, int64_t k, int64_t n, at::ScalarType t, at::ScalarType xt, int act) {
     fwa2_linear p = {};
@@ -161,6 +172,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &z = saved[2], &dy = grads[0];
+        refuse_unseen(dy);
         const int64_t how = ctx->saved_data["how"].toInt();
         const bool has_bias = how & 1, has_residual = how & 2;
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_bias && ctx->needs_input_grad(2),
@@ -189,6 +201,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& weight, const Optional& bias, int64_t act, const Optional& residual) {
+    refuse_unseen(x, weight, bias, residual);
     const Optional xo(x), wo(weight);
     if (wants_grad({&xo, &wo, &bias, &residual}))
         return LinearNode::apply(x, weight, bias, residual, act, act != FWA2_ACT_NONE && wants_grad({&xo, &wo, &bias}));
@@ -197,6 +210,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Optional& bias, int64
 
 Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& weight8, const Tensor& weight_scale, const Optional& bias, int64_t act,
                   const Optional& residual, bool bf16) {
+    refuse_unseen(x_scale, weight_scale, bias, residual);
     return linear_forward(x8, weight8, bias, (int)act, residual, bf16 ? at::kBFloat16 : at::kHalf, false, x_scale, weight_scale).first;
 }
 
@@ -285,6 +299,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         const bool has_s = code & 4, has_b = code & 8;
         const Tensor dy = how.pre() ? grads[1] : grads[0], dh = how.pre() ? grads[0] : Tensor();
         if (!dy.defined() && !dh.defined()) return variable_list(6);
+        refuse_unseen(dy, dh);
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1) && dy.defined(), need_s = has_s && ctx->needs_input_grad(2),
                    need_b = has_b && ctx->needs_input_grad(2 + has_s) && dy.defined();
         Tensor dx, ds, dw, db;
@@ -338,6 +353,7 @@ NormHow norm_how(const Tensor& x, const Optional& shortcut, double eps, int64_t 
 // [y] (post) or [h, y] (pre)
 variable_list norm(const Tensor& x, const Optional& shortcut, const Tensor& weight, const Optional& bias, double eps, int64_t kind, int64_t place,
                    const Optional& gate) {
+    refuse_unseen(x, shortcut, weight, bias, gate);
     const NormHow how = norm_how(x, shortcut, eps, kind, place);
     const Optional xo(x), wo(weight);
     if (wants_grad({&xo, &wo, &shortcut, &bias})) return NormNode::apply(x, weight, shortcut, bias, gate, how);
@@ -349,12 +365,14 @@ variable_list norm(const Tensor& x, const Optional& shortcut, const Tensor& weig
 // [stream, y8, scale]
 variable_list norm_fp8(const Tensor& x, const Optional& shortcut, const Tensor& weight, const Optional& bias, double eps, int64_t kind, int64_t place,
                        const Optional& gate) {
+    refuse_unseen(x, shortcut, weight, bias, gate);
     const NormHow how = norm_how(x, shortcut, eps, kind, place);
     const NormOut o = norm_forward(x, shortcut, weight, bias, gate, how, false, true);
     return {how.pre() ? o.h : o.y, o.y8, o.scale};
 }
 
 std::pair<Tensor, Tensor> quantize_rows(const Tensor& x) {
+    refuse_unseen(x);
     at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x.device());
     Tensor x8 = make(x.sizes(), x, at::kFloat8_e4m3fn), scale = make(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
