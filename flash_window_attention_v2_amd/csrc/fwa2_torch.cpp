@@ -10,8 +10,10 @@
 
 #include <ATen/FuncTorchTLS.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/fwa2.h"
 
@@ -98,12 +100,15 @@ bool wants_grad(std::initializer_list<const Optional*> ts) {
 }
 
 // What follows a computation from outside does not see into these functions.  A backward pass is recorded by their nodes; a
-// forward-mode derivative that an input carries would be lost, and so would what the transforms of torch.func keep.
+// forward-mode derivative that an input carries would be lost, and so would what the transforms of torch.func keep; a tracer
+// would record that an output is allocated and not what fills it.
 bool has_forward_grad(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_forward_grad(const Optional& t) { return t.has_value() && has_forward_grad(*t); }
 template <class... T>
 void refuse_unseen(const T&... ts) {
     if ((has_forward_grad(ts) || ...)) throw StatusError(FWA2_ERR_UNSUPPORTED, "the operator has no forward-mode derivative");
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+        throw StatusError(FWA2_ERR_UNSUPPORTED, "the operator cannot be traced");
     if (const auto& transforms = at::functorch::functorchTLSAccessor()) transforms->checkSupportsCppAutogradFunction();
 }
 

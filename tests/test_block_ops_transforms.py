@@ -86,3 +86,25 @@ def test_transforms_of_torch_func_are_refused(ext, name):
         torch.func.grad(lambda *a: first(*a).float().sum())(*args)
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.vmap(lambda a: first(a, *args[1:]))(torch.stack([args[0], args[0]]))
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("recorded", [False, True])
+def test_tracers_are_refused(ext, name, recorded):
+    """A trace would hold the output's allocation and not what fills it."""
+    make, args = CALLS[name]
+    call = make(ext)
+    if recorded:
+        if name in ("linear_fp8", "norm_fp8", "quantize_rows"):
+            return
+        args = tuple(a.clone().requires_grad_(i < 2) for i, a in enumerate(args))
+
+    def first(*a):
+        out = call(*a)
+        return out if isinstance(out, torch.Tensor) else out[0]
+
+    with pytest.raises((NotImplementedError, RuntimeError), match="trace"):
+        torch.jit.trace(first, args, check_trace=False)
+    with pytest.raises((NotImplementedError, RuntimeError), match="trace"):
+        make_fx(first)(*(a.detach() for a in args))
+    assert first(*args).shape[0] == 0           # afterwards as before
