@@ -70,6 +70,13 @@ def _hooked(*modules):
                or "forward" in m.__dict__ for m in modules)
 
 
+def _followed():
+    """Whether something follows the computation that the library's calls refuse: a tracer, a forward-mode derivative, a
+    transform of torch.func."""
+    return (torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+            or torch.autograd.forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active())
+
+
 class Mlp(nn.Module):
     """fc1, activation, fc2.  With `is_fused` the products run on the library's kernels (the activation in the epilogue of
     the first) wherever those apply: on the GPU in half precision, without active dropout, with an activation the library
@@ -105,7 +112,7 @@ class Mlp(nn.Module):
             return None
         if type(self.fc1) is not nn.Linear or type(self.fc2) is not nn.Linear or self._drops():
             return None
-        if _hooked(self.fc1, self.act, self.fc2, self.drop):
+        if _hooked(self.fc1, self.act, self.fc2, self.drop) or _followed():
             return None
         dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else x.dtype
         if dtype not in (torch.float16, torch.bfloat16):
@@ -442,7 +449,9 @@ class SwinTransformerBlock(nn.Module):
         """Whether shortcut + drop_path(norm(x)) runs as the library's one call, with the framework's types."""
         if not (self.is_fused and type(norm) is nn.LayerNorm and norm.weight is not None and x.is_cuda):
             return False
-        if type(self.drop_path) not in (DropPath, nn.Identity) or _hooked(norm, self.drop_path) or x.shape[-1] > 16384:
+        if type(self.drop_path) not in (DropPath, nn.Identity) or _hooked(norm, self.drop_path) or _followed():
+            return False
+        if x.shape[-1] > 16384:
             return False
         if norm.normalized_shape != (x.shape[-1],) or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             return False

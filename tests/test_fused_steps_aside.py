@@ -172,6 +172,30 @@ def test_an_eps_that_the_kernels_refuse_steps_aside():
         assert _fits(blk) == (True, True, True)
 
 
+def test_tracers_and_transforms_get_the_modules():
+    """The functions refuse these; the block's modules know how to go along."""
+    import torch.autograd.forward_ad as fwAD
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    seen, blk = [], _fused_block()
+
+    def look(x):
+        seen.append(_fits(blk))
+        return x * 2
+
+    x = torch.ones(3)
+    torch.jit.trace(look, x, check_trace=False)
+    make_fx(look)(x)
+    with fwAD.dual_level():
+        look(x)
+    torch.func.jvp(look, (x,), (x,))
+    torch.func.vmap(look)(x)
+    assert seen and set(seen) == {(False, False, False)}
+    seen.clear()
+    look(x)
+    assert seen == [(True, True, True)]
+
+
 # ---- held 8-bit weights ------------------------------------------------------------------------------------------------
 @pytest.fixture
 def holding(monkeypatch):
