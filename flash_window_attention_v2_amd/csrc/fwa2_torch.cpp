@@ -55,6 +55,10 @@ int64_t row_count(const Tensor& t) {
     return n;
 }
 
+// The tensor itself, unless it is a view that negates what its memory holds (the imaginary part of a conjugate is one).
+Tensor as_held(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor dense(const Tensor& t) { return as_held(t).contiguous(); }
+
 // A tensor as [rows, last] with unit inner stride: itself where the kernels can address it, a copy otherwise (inner stride
 // other than 1, rows that overlap or lie 2^22 elements apart or more).  The tensor lives as long as this does.
 struct Rows {
@@ -62,7 +66,7 @@ struct Rows {
     void* ptr = nullptr;
     int64_t stride = 0;
     Rows() = default;
-    explicit Rows(const Tensor& from) : t(from) {
+    explicit Rows(const Tensor& from) : t(as_held(from)) {
         const int64_t last = t.size(-1);
         stride = last;
         if (!t.is_contiguous()) {
@@ -155,10 +159,10 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& weight, 
     Rows rr;
     fwa2_linear p = linear_description(xr, wr, rows, k, n, t, x.scalar_type(), act);
     Tensor b, xs, ws;
-    if (bias) { b = bias->contiguous(); p.bias = b.data_ptr(); }
+    if (bias) { b = dense(*bias); p.bias = b.data_ptr(); }
     if (residual) { rr = Rows(*residual); p.residual = rr.ptr; p.residual_stride = rr.stride; }
     if (x_scale) {
-        xs = x_scale->contiguous(); ws = w_scale->contiguous();
+        xs = dense(*x_scale); ws = dense(*w_scale);
         p.x_scale = xs.data_ptr<float>(); p.weight_scale = ws.data_ptr<float>();
     }
     p.y = ptr(y); p.z = ptr(z);
@@ -241,11 +245,11 @@ fwa2_norm norm_description(const Tensor& v, const NormHow& how, const Tensor& we
     p.rows = row_count(v);
     TORCH_CHECK(v.size(-1) <= INT32_MAX, "norm: rows of more than 2^31 values");
     p.dim = (int)v.size(-1);
-    keep.weight = weight.contiguous();
+    keep.weight = dense(weight);
     p.weight = keep.weight.data_ptr();
-    if (bias.defined()) { keep.bias = bias.contiguous(); p.bias = keep.bias.data_ptr(); }
+    if (bias.defined()) { keep.bias = dense(bias); p.bias = keep.bias.data_ptr(); }
     if (gate.defined()) {
-        keep.gate = gate.contiguous();
+        keep.gate = dense(gate);
         p.gate = keep.gate.data_ptr();
         p.gate_dtype = dtype_code(gate.scalar_type());
         p.rows_per_gate = p.rows / gate.numel();

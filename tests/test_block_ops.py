@@ -244,3 +244,15 @@ def test_struct_sizes_match_the_header(lib):
         p.struct_bytes = 1
         check(ctypes.byref(p), 0)
         assert f"library {size} bytes" in lib.fwa2_last_error().decode()
+
+
+def test_rows_of_lazily_negated_views_are_negated(lib):
+    # the imaginary part of a conjugate: a real tensor whose memory holds the negated values
+    z = torch.randn(3, 8, dtype=torch.complex64)
+    neg = z.conj().imag
+    assert neg.is_neg()
+    rows, stride = _abi.load_ext().rows(neg)
+    assert not rows.is_neg() and torch.equal(rows, -z.imag) and stride == 8
+    dense = torch._neg_view(torch.randn(3, 8))
+    rows, stride = _abi.load_ext().rows(dense)
+    assert not rows.is_neg() and torch.equal(rows, dense) and stride == 8
