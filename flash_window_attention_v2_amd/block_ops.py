@@ -61,7 +61,7 @@ def _check_norm(x, shortcut, weight, bias, eps, kind, placement, gate):
         assert bias.shape == (dim,) and bias.dtype == weight.dtype, "bias must have the shape and dtype of weight"
     if gate is not None:
         assert gate.dtype in (x.dtype, torch.float32), "gate must be of the dtype of x or fp32"
-        assert gate.numel() > 0 and _count(x) % gate.numel() == 0, \
+        assert _count(x) == 0 or (gate.numel() > 0 and _count(x) % gate.numel() == 0), \
             "gate must hold one factor per sample: the rows of x must be a multiple of its size"
         assert not (torch.is_grad_enabled() and gate.requires_grad), "gate gets no gradient"
     if dim > _abi.NORM_MAX_DIM:

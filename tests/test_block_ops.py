@@ -256,3 +256,24 @@ def test_rows_of_lazily_negated_views_are_negated(lib):
     dense = torch._neg_view(torch.randn(3, 8))
     rows, stride = _abi.load_ext().rows(dense)
     assert not rows.is_neg() and torch.equal(rows, dense) and stride == 8
+
+
+@pytest.mark.parametrize("placement", ["post", "pre"])
+def test_no_rows_and_no_gates(lib, monkeypatch, placement):
+    # a batch of no samples under stochastic depth: no factors either, and empty results (no kernel runs: the CPU will do)
+    from flash_window_attention_v2_amd import block_ops
+
+    monkeypatch.setattr(block_ops, "_same_device", lambda *a: None)
+    x, w = torch.empty(0, 5, 8, requires_grad=True), torch.ones(8, requires_grad=True)
+    gate = torch.empty(0, 1, 1)
+    out = fwa2.residual_norm_func(x, x, w, w, placement=placement, gate=gate)
+    for t in out if placement == "pre" else (out,):
+        assert t.shape == x.shape
+    (out[1] if placement == "pre" else out).sum().backward()
+    assert x.grad.shape == x.shape and (w.grad == 0).all()
+    with torch.no_grad():
+        assert fwa2.residual_norm_fp8_func(x, x, w, w, placement=placement, gate=gate)[1].shape == x.shape
+    with pytest.raises(AssertionError, match="one factor per sample"):
+        fwa2.residual_norm_func(torch.ones(4, 8), None, w, gate=torch.empty(0))
+    with pytest.raises(AssertionError, match="one factor per sample"):
+        fwa2.residual_norm_func(torch.ones(4, 8), None, w, gate=torch.ones(3))
