@@ -1180,14 +1180,15 @@ static void launch_rows(const LinArgs& a, int cus, hipStream_t st) {
     else hipLaunchKernelGGL((linear_rows_kernel<DT, 2>), dim3(columns, (groups + 1) / 2), block, 0, st, a);
 }
 
-// The activations a product is compiled for; the others are decided at run time, row by row of the epilogue.
+// The activations a product is compiled for; the others are decided at run time, row by row of the epilogue.  The form without
+// an activation writes no z, which is then the same as y but for the residual: who asks for it gets the run-time form.
 template <int DT>
 static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, int cus, hipStream_t st) {
     if (vec && takes_rows(a.nq, a.np, cus)) {
         launch_rows<DT>(a, cus, st);
         return;
     }
-    if (a.act == FWA2_ACT_NONE) launch_product<DT, false, false, FWA2_ACT_NONE>(a, pl, vec, st);
+    if (a.act == FWA2_ACT_NONE && a.z == nullptr) launch_product<DT, false, false, FWA2_ACT_NONE>(a, pl, vec, st);
     else if (a.act == FWA2_ACT_GELU) launch_product<DT, false, false, FWA2_ACT_GELU>(a, pl, vec, st);
     else launch_product<DT, false, false, -1>(a, pl, vec, st);
 }
