@@ -8,6 +8,8 @@ import torch
 
 import flash_window_attention_v2_amd as fwa2
 from flash_window_attention_v2_amd import _abi
+from block_ops_exact import constant_rows, constant_rows_bound, layer, layer_sums
+from block_ops_ref import slope64
 
 FAKE = 0x100000     # never dereferenced by a validation
 
@@ -277,3 +279,32 @@ def test_no_rows_and_no_gates(lib, monkeypatch, placement):
         fwa2.residual_norm_func(torch.ones(4, 8), None, w, gate=torch.empty(0))
     with pytest.raises(AssertionError, match="one factor per sample"):
         fwa2.residual_norm_func(torch.ones(4, 8), None, w, gate=torch.ones(3))
+
+
+# ---- the inputs of the exact sums, with mistakes planted in the oracle ---------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,stretch", [(70000, 8, 8, 320), (16500, 64, 136, 320), (16500, 64, 136, 65), (5000, 96, 96, 20)])
+def test_exact_sums_show_a_lost_or_doubled_partial(m, k, n, stretch, dtype):
+    x, w, b, dy = layer(m, k, n, dtype, "cpu", m)
+    for act in (None, "relu"):
+        sums = layer_sums(x, w, b, dy, act)
+        want = {name: t.to(dtype) for name, t in sums.items()}
+        for lo in range(0, m, stretch):
+            part = layer_sums(x[lo:lo + stretch], w, b, dy[lo:lo + stretch], act)
+            for name in ("dw", "db"):
+                for sign in (-1, 1):
+                    assert not torch.equal((sums[name] + sign * part[name]).to(dtype), want[name]), (act, name, lo)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_constant_rows_show_rounded_gradients(act, dtype):
+    # the bound that dbias is held to refuses sums of dz rounded to dtype, and takes sums in fp32
+    m, n = 300, 512
+    z, dy = constant_rows(act, n, dtype, "cpu", 3)
+    dz = dy.double() * slope64(z.double(), act)
+    bound = constant_rows_bound(m * dz, m, dtype)
+    good = dz.float().expand(m, n).sum(0).to(dtype).double()
+    assert ((good - m * dz).abs() <= bound).all()
+    rounded_first = dz.to(dtype).float().expand(m, n).sum(0).to(dtype).double()
+    assert int(((rounded_first - m * dz).abs() > bound).sum()) > n // 10
