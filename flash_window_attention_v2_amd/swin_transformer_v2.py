@@ -120,6 +120,8 @@ class Mlp(nn.Module):
         params = [p for m in (self.fc1, self.fc2) for p in (m.weight, m.bias) if p is not None]
         if not torch.is_autocast_enabled() and any(p.dtype != dtype for p in params):
             return None
+        if x.dtype == torch.float64 or any(p.dtype == torch.float64 for p in params):      # which autocast leaves alone
+            return None
         return dtype
 
     def fp8_ready(self, x):

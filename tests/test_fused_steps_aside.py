@@ -196,6 +196,18 @@ def test_tracers_and_transforms_get_the_modules():
     assert seen == [(True, True, True)]
 
 
+def test_double_precision_under_autocast_keeps_the_modules(monkeypatch):
+    # autocast leaves fp64 alone
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda: True)
+    x = OnGpu()
+    x.dtype = torch.float32
+    mlp = _mlp().float()
+    assert mlp.fused_dtype(x) is torch.get_autocast_dtype("cuda")
+    assert mlp.double().fused_dtype(x) is None
+    x.dtype = torch.float64
+    assert mlp.fused_dtype(x) is None and mlp.float().fused_dtype(x) is None
+
+
 # ---- held 8-bit weights ------------------------------------------------------------------------------------------------
 @pytest.fixture
 def holding(monkeypatch):
