@@ -70,6 +70,11 @@ def _hooked(*modules):
                or "forward" in m.__dict__ for m in modules)
 
 
+def _plain(*parameters):
+    """Whether the parameters are nothing but values in memory: sharded and quantised ones are tensors of other classes."""
+    return all(p is None or type(p) in (nn.Parameter, torch.Tensor) for p in parameters)
+
+
 def _followed():
     """Whether something follows the computation that the library's calls refuse: a tracer, a forward-mode derivative, a
     transform of torch.func."""
@@ -118,6 +123,8 @@ class Mlp(nn.Module):
         if dtype not in (torch.float16, torch.bfloat16):
             return None
         params = [p for m in (self.fc1, self.fc2) for p in (m.weight, m.bias) if p is not None]
+        if not _plain(*params):
+            return None
         if not torch.is_autocast_enabled() and any(p.dtype != dtype for p in params):
             return None
         if x.dtype == torch.float64 or any(p.dtype == torch.float64 for p in params):      # which autocast leaves alone
@@ -453,7 +460,7 @@ class SwinTransformerBlock(nn.Module):
             return False
         if type(self.drop_path) not in (DropPath, nn.Identity) or _hooked(norm, self.drop_path) or _followed():
             return False
-        if x.shape[-1] > 16384:
+        if x.shape[-1] > 16384 or not _plain(norm.weight, norm.bias):
             return False
         if norm.normalized_shape != (x.shape[-1],) or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             return False

@@ -208,6 +208,26 @@ def test_double_precision_under_autocast_keeps_the_modules(monkeypatch):
     assert mlp.fused_dtype(x) is None and mlp.float().fused_dtype(x) is None
 
 
+class Wrapped(torch.Tensor):
+    """A weight that holds its values in a way of its own, as sharded and quantised ones do."""
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+def test_parameters_of_other_classes_keep_the_modules():
+    for part, want in (("mlp.fc1", (True, False, True)), ("mlp.fc2", (True, False, True)), ("norm1", (False, True, True)),
+                       ("norm2", (True, True, False))):
+        for name in ("weight", "bias"):
+            blk = _fused_block()
+            m = blk.get_submodule(part)
+            wrapped = nn.Parameter(getattr(m, name).detach().as_subclass(Wrapped))
+            del m._parameters[name]
+            m._parameters[name] = wrapped
+            assert type(getattr(m, name)) is Wrapped and _fits(blk) == want, (part, name)
+
+
 # ---- held 8-bit weights ------------------------------------------------------------------------------------------------
 @pytest.fixture
 def holding(monkeypatch):
