@@ -308,3 +308,18 @@ def test_held_weights_on_the_gpu_after_replacements():
             got = mlp(x)
             mlp.hold_weights8(False)
             assert torch.equal(mlp(x), got) and not torch.equal(got, held)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("is_fused", [False, True])
+def test_a_compiled_block_runs(is_fused):
+    """A graph compiler breaks its graph at the library's calls and gives the same numbers."""
+    blk = _block(is_fused=is_fused, fp8_mlp=is_fused).cuda().to(torch.bfloat16).eval()
+    x = torch.randn(2, 64, 16, device="cuda", dtype=torch.bfloat16)
+    compiled = torch.compile(blk, backend="eager")
+    with torch.no_grad():
+        assert torch.equal(compiled(x), blk(x))
+    leaf, twin = x.clone().requires_grad_(), x.clone().requires_grad_()
+    compiled(leaf).sum().backward()
+    blk(twin).sum().backward()
+    assert torch.equal(leaf.grad, twin.grad)
