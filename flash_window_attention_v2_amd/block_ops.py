@@ -11,7 +11,8 @@ Tensors of any strides are taken; what the kernels cannot address (an inner stri
 2^22 elements apart or more) is copied first.  Leading dimensions are flattened to rows.  Every call works on the current
 stream of the tensors' device and can be captured into a graph (a backward pass, as with any autograd operator: while no
 eager graph of the same leaves is alive, whose nodes belong to another stream); gradients are bit-reproducible and
-cannot be differentiated a second time (that raises).
+cannot be differentiated a second time (that raises).  Inputs that carry a forward-mode derivative, the transforms of
+torch.func and tracers are refused (NotImplementedError or RuntimeError): they would not see what happens in here.
 """
 import torch
 

@@ -18,11 +18,12 @@
 // partial tiles are added in a fixed order by a second kernel.  dbias is the same contraction against ones and rides on the
 // matrix pipe of the workgroups with the first column tile.
 //
-// What bounds it, measured on MI355X.  Short contractions: memory.  262144 x 96 -> 384 with GELU 66 us for 252 MB
-// (3.8 TB/s; a large copy reaches 5.2, and the stores queue behind a tile's loads); 65536 x 768 -> 192 with a residual 33 us
-// (4.6 TB/s).  Long ones: the matrix pipe.  8192 x 4096 -> 4096 bf16 242 us = 1 137 TFLOP/s (the library's plain product of
-// that size 212 us), 8-bit 129 us = 2 130 TFLOP/s.  Between the two every product of a training step sits near both limits:
-// 16384 x 384 -> 1536, forward with z 38 us (2.9 TB/s), dx 28 us, dW 31 + 10 us.
+// What bounds it, measured on MI355X kernel by kernel under a profiler, two sets of inputs in turn.  Short contractions:
+// memory.  262144 x 96 -> 384 with GELU 66 us for 252 MB (3.8 TB/s; a large copy reaches 5.1, and the stores queue behind a
+// tile's loads); 65536 x 768 -> 192 with a residual 34 us (4.4 TB/s).  Long ones: the matrix pipe.  8192 x 4096 -> 4096 bf16
+// 258 us = 1 066 TFLOP/s (back to back without the profiler 246; the library's plain product of that size 205), 8-bit 139 to
+// 147 us, up to 1 980 TFLOP/s; the pipe is busy 59 % and 51 % of these.  Between the two every product of a training step sits
+// near both limits: 16384 x 384 -> 1536, forward with z 40 us (2.8 TB/s), dx 29 us, dW 34 + 10 us.
 #include <initializer_list>
 #include <type_traits>
 
@@ -72,7 +73,7 @@ template <> struct LinElem<FWA2_E4M3> { static constexpr int bytes = 1; };
 // over the fit, and falls on beyond it (6e-16 at 8, 0 from 20 on, where u is cut so that infinity meets a zero).  Eight
 // instructions and one exponential: the library's erff takes about 40, which in the epilogue of a product with few
 // contraction elements (262144 x 96 -> 384) are 130 us of vector instructions next to 49 us of memory traffic; the whole
-// call now takes 66.
+// kernel now takes 66.
 __device__ __forceinline__ float normal_tail(float u) {
     float p = -1.1775869097618852e-06f;
     p = __builtin_fmaf(p, u, 4.9426900659454986e-05f);
@@ -953,7 +954,11 @@ __global__ void __launch_bounds__(64 * W) linear_sum_kernel(const float* part, i
 
 // dz = dy act'(z), contiguous, and the column sums of dz before its rounding (part_db, one partial row per blockIdx.y).
 // A workgroup owns up to 512 columns (8 per lane, `lanes` lanes a row, a power of two) and a stretch of rows; bound by its
-// three streams (16384 x 1536: 30 us, 5.0 TB/s).
+// three streams (16384 x 1536: 32 us, 4.7 TB/s).
+//
+// dz leaves in the element type because it is an operand of the matrix products behind, which take 16 bits: with the
+// result's own rounding dx and dW are then 0.0024 off in bf16 (2-norm, 16384 x 384 -> 1536 with GELU), where sums of unrounded
+// dz rounded once would be 0.0017 off.  z is kept in it too: in 32 bits it would move 100 MB more beside that case's 243.
 constexpr int kActRows = 256;      // at most so many stretches of rows: their partial sums stay small
 template <class E, int ACT, bool VEC>
 __global__ void __launch_bounds__(256) act_backward_kernel(const E* dy, int64_t dy_stride, const E* z, E* dz, int64_t rows,
@@ -1065,24 +1070,33 @@ struct LinPlan {
     int tiles_p;
 };
 
-// The rule, with what it was measured on (MI355X, us, bf16, operands not in the caches; rows x contraction -> columns):
-//   262144 x   96 ->  384 gelu       T128S  62, T128  94, T192P 106, T256 115, T64  94
-//    65536 x  192 ->  768 gelu, z    T128S  62, T128  67, T192P  65, T256P  58
-//    65536 x  192 ->  768 (dx)       T128S  49, T128  49, T192P  44, T256P  38
-//    16384 x  384 -> 1536 gelu, z    T128S  40, T128  38, T192P  39, T256  44, T64  55
-//    65536 x  768 ->  192 residual   T128S  39, T128  33, T192P  26, T256  32, T64  57
-//     4096 x  768 -> 1536 gelu, z    T128S  28, T128  25, T192P  24,           T64  27
-//     4096 x 1536 ->  768 residual   T128S  28, T128  21, T192P  25,           T64  22     (T192P: half the CUs)
-//    16384 x  384 ->  384            T128S  13, T128  11, T192P  11,           T64  14
-//    16384 x  384 ->   96 residual   T128S   9, T128   8, T192P  10,           T64   7
-//     2048 x 1024 -> 1024            T128S  15, T128  14,                      T64  11
-//      512 x 4096 -> 1024            T128S  45, T128  43,                      T64  25
-//     8192 x 4096 -> 4096 residual   T128S 375, T128 291, T192P 283, T256 228, T64 665
-// weight gradients (rows of dW x rows of the batch -> columns of dW), splits chosen as below:
-//      384 x 262144 ->  96           T128  49, T192Q 39, T192P 64, T192 50, T256  65
-//     1536 x  16384 -> 384           T128  35, T192Q 36, T192P 36, T192 30, T256  53
-//      192 x  65536 -> 768           T128  42, T192Q 35, T192P 31, T192 30, T256  52
-//     4096 x   8192 -> 4096          T128 287, T192Q 274, T192P 275, T192 278, T256 216
+// The rule, with what it was measured on (MI355X, us, bf16, launches back to back whose operands and results move through
+// 1 GB, so that the caches hold none of them; rows x contraction -> columns):
+//   262144 x   96 ->  384 gelu       T128S  85, T128  92, T192P  91, T256 109, T256P  94, T64 133
+//    65536 x  192 ->  768 gelu, z    T128S  64, T128  69,                      T256P  59
+//    65536 x  192 ->  768 (dx)       T128S  42, T128  44,                      T256P  39
+//    16384 x  384 -> 1536 gelu, z    T128S  42, T128  36, T192P  37, T256  46,           T64  49
+//    16384 x 1536 ->  384 (dx)       T128S  35, T128  30, T192P  30, T256  42,           T64  41
+//    65536 x  768 ->  192 residual   T128S  54, T128  40, T192P  32, T256  34,           T64  52
+//     4096 x  768 -> 1536 gelu, z    T128S  24, T128  21, T192P  22,                     T64  26
+//     4096 x 1536 ->  768 residual   T128S  31, T128  26, T192P  29,                     T64  23     (T192P: half the CUs)
+//    16384 x  384 ->  384            T128S  14, T128  12, T192P  12,                     T64  15
+//    16384 x  384 ->   96 residual   T128S  11, T128  10, T192P  11,                     T64   7
+//     2048 x 1024 -> 1024            T128S  17, T128  13,                                T64  10
+//      512 x 4096 -> 1024            T128S  56, T128  42,                                T64  24
+//     8192 x 4096 -> 4096 residual   T128S 378, T128 313, T192P 286, T256 238,           T64 593
+// T256P on both sides of its borders (T128S or T128, whichever the rule would take / T256P; forward with gelu and z, dx):
+//   contraction, 65536 rows, 768 columns:  88: 47 / 46, 28 / 24    96: 49 / 45, 30 / 24   104: 54 / 48, 34 / 27
+//                                         192: 64 / 59, 42 / 39   200: 75 / 66, 51 / 43   208: 75 / 65, 51 / 43
+//   workgroups, contraction 192:          192: 9.4 / 9.8, 9.1 / 9.7    384: 14 / 14, 13 / 14   (one row of tiles short of) 512:
+//                                         19 / 15, 18 / 18   513: 19 / 22, 19 / 20   768: 25 / 24, 24 / 23   1023: 34 / 29, 32 / 28
+//   columns, 65536 rows:                  256: 22 / 17   384: 26 / 27 (a third of its tiles' columns empty)   512: 31 / 27
+// so it would pay from 88 to 208 elements as well; below two workgroups to a CU it does not.
+// weight gradients (rows of dW x rows of the batch -> columns of dW), splits chosen as below, without the sum behind:
+//      384 x 262144 ->  96           T128  56, T192Q  51, T192P  57, T192  56
+//     1536 x  16384 -> 384           T128  41, T192Q  34, T192P  37, T192  36
+//      192 x  65536 -> 768           T128  51, T192Q  37, T192P  40, T192  43
+//     4096 x   8192 -> 4096          T128 332, T192Q 306, T192P 314, T192 314, T256 225
 static LinPlan plan_product(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
     auto up = [](int64_t n, int b) { return (n + b - 1) / b; };
     auto count = [&](Tile t) { return up(nq, kTiles[t].bq) * up(np, kTiles[t].bp); };
@@ -1161,17 +1175,17 @@ static void launch_product(LinArgs a, const LinPlan& pl, bool vec, hipStream_t s
 
 // Which products linear_rows_kernel takes: up to 16 rows, and any number whose workgroups find a CU each; beyond that the
 // gathering of x costs more than the 64 x 64 tiles' stages, one after the other, do.  Measured (bf16, us, tiles / this
-// kernel, cold weights):
-//     1 x  768 ->  1536   8.2 / 4.5      64 x  768 -> 1536   6.8 /  4.9      256 x 1536 ->  384  10.8 /  6.9
-//     1 x 4096 ->  4096  28.1 / 8.7      64 x 4096 -> 1024  23.9 / 10.3      128 x 4096 -> 1024  24.2 / 13.4
-//     1 x 1024 -> 16384  10.3 / 8.3      16 x 1024 -> 16384 10.8 / 11.1       16 x  384 -> 8192   4.6 /  4.3
-// and beyond the rule:                   32 x 1024 -> 16384 11.2 / 16.0      256 x  768 -> 1536   6.9 /  9.5
-//                                        64 x 4096 ->  4096 28.6 / 25.5      128 x 4096 -> 4096  28.9 / 46.6
+// kernel, launches back to back with weights that the caches do not hold):
+//     1 x  768 ->  1536   9.2 / 5.0      64 x  768 -> 1536   6.8 /  4.7      256 x 1536 ->  384  10.8 /  6.8
+//     1 x 4096 ->  4096  28.3 / 9.1      64 x 4096 -> 1024  26.8 / 10.8      128 x 4096 -> 1024  27.1 / 14.7
+//     1 x 1024 -> 16384  10.1 / 8.4      16 x 1024 -> 16384 11.0 / 11.5       16 x  384 -> 8192   4.7 /  4.3
+// and beyond the rule:                   32 x 1024 -> 16384 11.0 / 16.1      256 x  768 -> 1536   6.8 /  9.4
+//                                        64 x 4096 ->  4096 28.8 / 26.0      128 x 4096 -> 4096  29.1 / 46.6
 static bool takes_rows(int64_t nq, int np, int cus) {
     return nq <= 16 || ((nq + 31) / 32) * (int64_t)((np + 15) / 16) <= cus;
 }
-// 16 rows to a workgroup while there is a CU for each, 32 otherwise (64 x 4096 -> 1024: 10.2 / 13.3 us; -> 4096: 32.6 / 25.6);
-// 8 wavefronts, 4 where there are many workgroups (1 x 1024 -> 16384: 8.2 us with 4, 9.8 with 8, 14.1 with 16).
+// 16 rows to a workgroup while there is a CU for each, 32 otherwise (64 x 4096 -> 1024: 10.9 / 14.5 us; -> 4096: 32.8 / 25.8);
+// 8 wavefronts, 4 where there are many workgroups (1 x 1024 -> 16384: 8.4 us with 4, 9.9 with 8; 1 x 4096 -> 4096: 12.0 / 9.1).
 template <int DT>
 static void launch_rows(const LinArgs& a, int cus, hipStream_t st) {
     const int64_t columns = (a.np + 15) / 16, groups = (a.nq + 15) / 16;
@@ -1194,8 +1208,9 @@ static void launch_forward(const LinArgs& a, const LinPlan& pl, bool vec, int cu
 }
 
 // Tiles for operands that go through registers: 128 wide when those fill the chip twice (their loads are waited for stage by
-// stage, so there have to be several workgroups to a CU), 64 otherwise.  Measured (us, 64 / 128 wide): 1225 x 588 -> 333
-// 10.6 / 17.7 and its weight gradient 10.9 / 13.2; 4099 x 585 -> 1161 25.9 / 23.8, 40.9 / 50.6; 16389 x 585 -> 1161 97 / 63.
+// stage, so there have to be several workgroups to a CU), 64 otherwise.  Measured (us, 64 / 128 wide, operands not in the
+// caches): 1225 x 588 -> 333 13.9 / 18.9 and its weight gradient 11.3 / 13.4; 4099 x 585 -> 1161 27.1 / 23.7, 43.4 / 51.0;
+// 16389 x 585 -> 1161 96.7 / 64.2.
 static LinPlan plan_unaligned(int64_t nq, int np, int64_t nk, bool split, int elem_bytes, int cus) {
     LinPlan pl;
     auto count = [&](int b) { return ((nq + b - 1) / b) * ((np + b - 1) / b); };
@@ -1224,9 +1239,10 @@ static inline bool rows16(const void* p, int64_t stride, int64_t len, int bytes)
 
 // Results too large to be found in the 256 MB memory-side cache by whoever reads them next leave with non-temporal stores: plain
 // ones fill the L2s with lines that wait to be written back, behind which the operands of the next tiles queue.  Measured
-// (us, plain / non-temporal): 262144 x 96 -> 384 with GELU 90 / 65, without 80 / 45; 65536 x 192 -> 768 46 / 32;
-// 16384 x 384 -> 1536 with z 44 / 38.  An MLP whose second product reads the 201 MB of the first: 178 / 184 forward, but
-// 804 / 762 forward and backward.  Smaller results stay in the cache: 100 MB and less gained nothing in such a chain.
+// (us, plain / non-temporal), with two sets of operands in turn, which the cache keeps where the results do not push them out,
+// and with operands that no cache holds: 262144 x 96 -> 384 with GELU 90 / 73 and 90 / 85, without 75 / 45 and 77 / 73;
+// 65536 x 192 -> 768 38 / 34 and 41 / 40, with GELU and z 59 / 51 and 62 / 60; 16384 x 384 -> 1536 with both 37 / 36 and
+// 43 / 38.  An MLP whose second product reads the 201 MB of the first: 178 / 184 forward, but 804 / 762 forward and backward.
 static bool stream_results(int64_t rows, int columns, bool z) { return (double)rows * columns * (z ? 4 : 2) >= (64 << 20); }
 
 static LinArgs forward_args(const fwa2_linear* p) {

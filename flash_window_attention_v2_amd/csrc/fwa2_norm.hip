@@ -20,9 +20,11 @@
 // Its lanes keep their columns, so weight and bias are read once and the column sums dw, db stay in registers until the
 // end; one partial row per workgroup then goes to the workspace and a second kernel adds those in a fixed order.
 //
-// Measured on MI355X, where a large copy moves 5.2 TB/s: 262144 x 96 bf16 forward 36 us (4.3 TB/s), backward 38 us
-// (4.0 TB/s) and 5 us for the parameters' sums; 16384 x 1536 pre-norm with y, h and 8-bit rows 50 us (5.5 TB/s);
+// Measured on MI355X, where a large copy moves 5.1 TB/s: 262144 x 96 bf16 forward 36 us (4.3 TB/s), backward 37 us
+// (4.0 TB/s) and 5 us for the parameters' sums; 16384 x 1536 pre-norm with h in fp32 and 8-bit rows 49 us (5.7 TB/s);
 // 8-bit form of 8192 x 4096 bf16 16 us (6.3 TB/s, part of x still in the caches).  One row: 3 us, the launch itself.
+// 4099 x 385 fp16, pre-norm: forward 7 us; backward 14 us, one workgroup to a CU and four to five rounds of loads one after
+// the other (1.1 TB/s), and 4 us for the parameters' sums.
 #include <type_traits>
 
 #include "fwa2_common.hpp"
